@@ -51,6 +51,7 @@ typedef enum {
 typedef enum { TCG_ACC_F32 = 0, TCG_ACC_F16 = 1 } tcg_acc;
 typedef enum { TCG_B_KN = 0, TCG_B_NK = 1 } tcg_b_layout;
 typedef enum { TCG_F8_E4M3 = 0, TCG_F8_E5M2 = 1 } tcg_f8_format;
+typedef enum { TCG_F32 = 0, TCG_F16 = 1, TCG_BF16 = 2 } tcg_dtype;
 
 /* fp16 x fp16 -> fp32 C, fp32 (TCG_ACC_F32) or fp16 (TCG_ACC_F16) accumulation.
  * Replaces fp16 launch_kernel: kernels/fp16_wmma.cu:92-102 (fp32 acc) and
@@ -127,6 +128,67 @@ tcg_status tcg_gemm_s4_dequant(const int8_t* A_packed, const int8_t* BT_packed, 
 tcg_status tcg_quantize_absmax_s8(const float* src, int8_t* dst, size_t n, float* scale, void* stream);
 tcg_status tcg_quantize_absmax_s4(const float* src, int8_t* dst_packed, int rows, int cols_k, float* scale,
                                   void* stream);
+
+/* Absmax quantisation with one scale per row: rows x k values of `type` (row
+ * major) to int8 codes of the same layout and scale[rows] (device floats):
+ *   scale = max|x| / 127, code = round half away from zero (x * (1 / scale)),
+ * every step in IEEE single precision; a row of zeros has scale 0 and codes 0,
+ * a row with an infinity or NaN a scale that is not finite.  src and scale
+ * need their element's alignment only; rows of whole 16-byte vectors at a
+ * 16-byte aligned src take the faster path.  The left operand of the next
+ * three. */
+tcg_status tcg_quantize_rows_s8(const void* src, tcg_dtype type, int8_t* dst, float* scale, long long rows, int k,
+                                void* stream);
+
+/* Products of int8 rows with a scale each and int8 weights with a scale per
+ * output channel (B is N x K, "BT"):
+ *   C[m][n] = (float)(sum_k A[m][k] B[n][k]) * scale_a[m] * scale_b[n] + bias[n]
+ * rounded once to c_type.  scale_a: batches x M floats, scale_b and bias (or
+ * NULL): batches x N floats, on the device.  K % 16 == 0, A and B 16-byte
+ * aligned, C aligned to its element; M and N arbitrary.
+ * tcg_linear_s8 quantises its left operand itself (tcg_quantize_rows_s8) into
+ * `workspace` (tcg_linear_s8_workspace_size bytes, 256-byte aligned, not
+ * shared by calls that may overlap), then multiplies. */
+tcg_status tcg_gemm_s8_scaled(const int8_t* A, const int8_t* B, void* C, tcg_dtype c_type, int M, int N, int K,
+                              int batches, const float* scale_a, const float* scale_b, const float* bias,
+                              void* stream);
+size_t tcg_linear_s8_workspace_size(int M, int K);
+tcg_status tcg_linear_s8(const void* x, tcg_dtype x_type, const int8_t* B, void* C, tcg_dtype c_type, int M, int N,
+                         int K, const float* scale_b, const float* bias, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
+/* Products of grouped rows (one weight matrix per group, as a mixture of
+ * experts has): rows offsets[e] .. offsets[e + 1] - 1 of A meet matrix e of B.
+ * offsets: groups + 1 ascending row bounds on the device (0 < groups <=
+ * TCG_MAX_GROUPS), any of the groups empty; they are clamped to be ascending
+ * and within 0 .. M.  Rows of C outside every group are set to zero
+ * (zero_rest != 0) or left as they are.  NULL offsets: `groups` groups of
+ * M / groups rows each (M % groups == 0).
+ * tcg_gemm_16_grouped: A and B fp16 or bf16 (`type`), fp32 sums, C rounded once
+ * to c_type; B is groups x N x K (TCG_B_NK) or groups x K x N (TCG_B_KN); K % 8
+ * == 0 (and N % 8 == 0 for TCG_B_KN).  The gradient by A is the same product
+ * of the gradient by C with B in the other layout.
+ * tcg_gemm_16_grouped_wgrad: the gradient by B of the TCG_B_NK product:
+ *   dB[e][n][k] = sum over the rows m of group e of dC[m][n] * A[m][k]
+ * (zeros for an empty group), N % 8 == 0 and K % 8 == 0.  With scale_a, A holds
+ * int8 codes with a scale per row (tcg_quantize_rows_s8; K % 16 == 0) and
+ * stands for scale_a[m] * A[m][k] rounded to `type`.
+ * tcg_gemm_s8_grouped / tcg_linear_s8_grouped: as tcg_gemm_s8_scaled /
+ * tcg_linear_s8 with scale_b and bias groups x N. */
+#define TCG_MAX_GROUPS 1024
+tcg_status tcg_gemm_16_grouped(const void* A, const void* B, tcg_dtype type, void* C, tcg_dtype c_type,
+                               const int32_t* offsets, int groups, int M, int N, int K, tcg_b_layout b_layout,
+                               int zero_rest, void* stream);
+tcg_status tcg_gemm_16_grouped_wgrad(const void* dC, const void* A, const float* scale_a, tcg_dtype type, void* dB,
+                                     tcg_dtype b_type, const int32_t* offsets, int groups, int M, int N, int K,
+                                     void* stream);
+tcg_status tcg_gemm_s8_grouped(const int8_t* A, const int8_t* B, void* C, tcg_dtype c_type, const int32_t* offsets,
+                               int groups, int M, int N, int K, const float* scale_a, const float* scale_b,
+                               const float* bias, int zero_rest, void* stream);
+tcg_status tcg_linear_s8_grouped(const void* x, tcg_dtype x_type, const int8_t* B, void* C, tcg_dtype c_type,
+                                 const int32_t* offsets, int groups, int M, int N, int K, const float* scale_b,
+                                 const float* bias, int zero_rest, void* workspace, size_t workspace_bytes,
+                                 void* stream);
 
 /* Widen packed int4 to int8 (low nibble first), n_packed bytes -> 2*n_packed.
  * The first pass of tcg_gemm_s4's two-pass form, exposed for reuse. */
@@ -205,6 +267,12 @@ tcg_status tcg_selftest_wait_timeout(uint64_t timeout_ns, void* stream);
  * Shapes a precision cannot run fall back to the nearest valid one. */
 void tcg_set_tile_n(int bn);
 void tcg_set_cta_pair(int mode);
+
+/* The same for the scaled and grouped products above: the tile's rows (0 =
+ * automatic; 16, 32, 64 or 128 with 128 features, or 256 with 256; weight
+ * gradients take 128 or 256) and the CTAs that share a tile's sum (0 =
+ * automatic; 1, 2, 4 or 8; tiles of 256 rows take 1). */
+void tcg_set_rows_tile(int rows, int split);
 
 /* Introspection: last CUDA error code seen, status names, library version,
  * and the tile shape (width, rows) chosen by the most recent launch on this

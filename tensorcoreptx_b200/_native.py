@@ -17,6 +17,8 @@ TCG_SUCCESS = 0
 TCG_ERR_TIMEOUT = 3
 TCG_ACC_F32, TCG_ACC_F16 = 0, 1
 TCG_B_KN, TCG_B_NK = 0, 1
+TCG_F32, TCG_F16, TCG_BF16 = 0, 1, 2
+TCG_MAX_GROUPS = 1024
 
 STATUS_NAMES = {0: "TCG_SUCCESS", 1: "TCG_ERR_SHAPE", 2: "TCG_ERR_ALIGN", 3: "TCG_ERR_TIMEOUT",
                 4: "TCG_ERR_CUDA", 5: "TCG_ERR_ARG", 6: "TCG_ERR_UNSUPPORTED",
@@ -39,6 +41,14 @@ SIGNATURES = {
     "tcg_gemm_s4_dequant": (C.c_int, [_p, _p, _p, _i, _i, _i, _i, _p, _p, _p, _sz, _p]),
     "tcg_quantize_absmax_s8": (C.c_int, [_p, _p, _sz, _p, _p]),
     "tcg_quantize_absmax_s4": (C.c_int, [_p, _p, _i, _i, _p, _p]),
+    "tcg_quantize_rows_s8": (C.c_int, [_p, _i, _p, _p, C.c_longlong, _i, _p]),
+    "tcg_gemm_s8_scaled": (C.c_int, [_p, _p, _p, _i, _i, _i, _i, _i, _p, _p, _p, _p]),
+    "tcg_linear_s8_workspace_size": (_sz, [_i, _i]),
+    "tcg_linear_s8": (C.c_int, [_p, _i, _p, _p, _i, _i, _i, _i, _p, _p, _p, _sz, _p]),
+    "tcg_gemm_16_grouped": (C.c_int, [_p, _p, _i, _p, _i, _p, _i, _i, _i, _i, _i, _i, _p]),
+    "tcg_gemm_16_grouped_wgrad": (C.c_int, [_p, _p, _p, _i, _p, _i, _p, _i, _i, _i, _i, _p]),
+    "tcg_gemm_s8_grouped": (C.c_int, [_p, _p, _p, _i, _p, _i, _i, _i, _i, _p, _p, _p, _i, _p]),
+    "tcg_linear_s8_grouped": (C.c_int, [_p, _i, _p, _p, _i, _p, _i, _i, _i, _i, _p, _p, _i, _p, _sz, _p]),
     "tcg_gemm_s4_static": (C.c_int, [_p, _p, _p, _i, _i, _i, _i, _p]),
     "tcg_copy_2d_async": (C.c_int, [_p, _sz, _p, _sz, _sz, _sz, _p]),
     "tcg_host_register": (C.c_int, [_p, _sz]),
@@ -48,6 +58,7 @@ SIGNATURES = {
     "tcg_selftest_wait_timeout": (C.c_int, [C.c_uint64, _p]),
     "tcg_set_tile_n": (None, [_i]),
     "tcg_set_cta_pair": (None, [_i]),
+    "tcg_set_rows_tile": (None, [_i, _i]),
     "tcg_last_cuda_error": (C.c_int, []),
     "tcg_status_string": (C.c_char_p, [_i]),
     "tcg_version": (C.c_int, []),

@@ -35,7 +35,7 @@ def _sources(*names):
 
 
 def _deps():
-    return [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + \
+    return [os.path.join(CSRC, f) for f in os.listdir(CSRC) if not f.endswith(".o")] + \
         [os.path.join(INCLUDE, f) for f in os.listdir(INCLUDE)]
 
 
@@ -52,11 +52,40 @@ def _run(cmd, verbose):
     subprocess.check_call(cmd)
 
 
+def _includes(path, seen=None):
+    """The files of this tree that `path` includes, itself among them."""
+    seen = set() if seen is None else seen
+    if path not in seen and os.path.exists(path):
+        seen.add(path)
+        for line in open(path):
+            if line.startswith('#include "'):
+                _includes(os.path.normpath(os.path.join(os.path.dirname(path), line.split('"')[1])), seen)
+    return seen
+
+
+def _compile(names, force, verbose):
+    """Each source to an object file, those out of date side by side."""
+    objects, running = [], []
+    for src in _sources(*names):
+        obj = src[:-3] + ".o"
+        objects.append(obj)
+        if force or _stale(obj, sorted(_includes(src))):
+            cmd = [NVCC] + [f for f in COMMON if f != "-shared"] + ["-c", src, "-o", obj]
+            if verbose:
+                print(" ".join(cmd), flush=True)
+            running.append((cmd, subprocess.Popen(cmd)))
+    for cmd, p in running:
+        if p.wait() != 0:
+            raise subprocess.CalledProcessError(p.returncode, cmd)
+    return objects
+
+
 def build(force: bool = False, verbose: bool = True) -> list[str]:
     deps = _deps()
     built = []
     if force or _stale(LIB, deps):
-        _run([NVCC] + COMMON + _sources("tcgemm.cu") + ["-o", LIB], verbose)
+        objects = _compile(("tcgemm.cu", "tcg_rows.cu"), force, verbose)
+        _run([NVCC] + COMMON + objects + ["-o", LIB], verbose)
         built.append(LIB)
     defines = {"f16": "TCG_COMPAT_F16", "s8": "TCG_COMPAT_S8", "s4": "TCG_COMPAT_S4"}
     for prec, out in COMPAT.items():

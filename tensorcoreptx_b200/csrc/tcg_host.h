@@ -1,0 +1,40 @@
+// tcg_host.h -- host-side services that the library's translation units share
+// (defined in tcgemm.cu; take_rows_error in tcg_rows.cu).
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include "../../include/tcgemm.h"
+
+#pragma GCC visibility push(hidden)
+namespace tcg {
+namespace host {
+
+constexpr int kDevices = 64;
+
+// Record a CUDA error for tcg_last_cuda_error; returns TCG_ERR_CUDA.
+tcg_status fail(cudaError_t e);
+
+// The current device (TCG_ERR_UNSUPPORTED unless sm_100), its SM count, and
+// the driver's tensor-map encoder resolved.
+tcg_status device(int* id, int* sms);
+
+// A 3-D tiled tensor map: extents {d0 (contiguous), d1, d2}, byte strides of
+// d1 and d2, box {box0, box1, 1}.
+struct Box3 {
+    uint64_t d0, d1, d2, s1, s2;
+    uint32_t box0, box1;
+};
+tcg_status encode_3d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, const Box3& b,
+                     CUtensorMapSwizzle swz);
+
+bool dependent_launch();               // programmatic dependent launch (TCG_PDL)
+unsigned long long wait_timeout_ns();  // tcg_set_wait_timeout_ns
+
+// Read and clear the failure word of tcg_rows.cu's kernels on this device.
+tcg_status take_rows_error(unsigned long long* word);
+
+}  // namespace host
+}  // namespace tcg
+#pragma GCC visibility pop

@@ -17,6 +17,11 @@
 
 #include <cstdint>
 
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "tcg_ptx.cuh"
+
 namespace tcg {
 
 // |x| max over n floats into *absmax_bits (float bits, must start at +0).
@@ -131,6 +136,114 @@ __global__ void quantize_s4_kernel(const float* __restrict__ x, int8_t* __restri
     const float2* x2 = reinterpret_cast<const float2*>(x);
     for (long long j = n_g * 4 + static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; j < n_pairs; j += stride)
         out[j] = static_cast<int8_t>(quant_byte4(x2[j], inv));
+}
+
+// ---- one scale per row ----------------------------------------------------
+//
+// codes[m][k] and scale[m] of each row m of fp32, fp16 or bf16 values, by the
+// arithmetic above with Q = 127 and the row's own absmax.  kGroup threads (a
+// warp or a block) take a row.  The row is read once: up to kRowVecs 16-byte
+// vectors a thread stay in registers between the absmax and the codes; what is
+// longer is read again, from L2.  A row of zeros has scale 0 and codes 0.  The
+// absmax is taken on the bit patterns, where infinity and NaN are the largest:
+// such a row gets a scale that is not finite, and codes that dequantise to NaN.
+constexpr int kRowVecs = 8;
+constexpr int kRowThreads = 256;
+
+template <class T>
+__device__ __forceinline__ float row_value(T v) { return static_cast<float>(v); }
+
+// 16 bytes of a row as floats
+template <class T>
+struct RowVec {
+    static constexpr int kN = 16 / sizeof(T);
+    float f[kN];
+    __device__ __forceinline__ explicit RowVec(const uint4& v)
+    {
+        const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+        for (int i = 0; i < kN; ++i) f[i] = row_value(e[i]);
+    }
+};
+
+template <class T>
+__device__ __forceinline__ uint32_t row_absmax(const uint4& v, uint32_t m)
+{
+    const RowVec<T> x(v);
+#pragma unroll
+    for (int i = 0; i < RowVec<T>::kN; ++i) m = max(m, __float_as_uint(x.f[i]) & 0x7FFFFFFFu);
+    return m;
+}
+
+template <class T>
+__device__ __forceinline__ void row_codes(const uint4& v, float inv, int8_t* out)
+{
+    const RowVec<T> x(v);
+    uint32_t w[RowVec<T>::kN / 4];
+#pragma unroll
+    for (int i = 0; i < RowVec<T>::kN / 4; ++i)
+        w[i] = quant_word8(make_float4(x.f[4 * i], x.f[4 * i + 1], x.f[4 * i + 2], x.f[4 * i + 3]), inv);
+    if constexpr (RowVec<T>::kN == 8)
+        *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
+    else
+        *reinterpret_cast<uint32_t*>(out) = w[0];
+}
+
+// kVec: rows are whole 16-byte vectors (and dst takes their codes in one store)
+template <class T, int kGroup, bool kVec>
+__global__ void __launch_bounds__(kRowThreads)
+    quantize_rows_kernel(const T* __restrict__ x, int8_t* __restrict__ out, float* __restrict__ scale, long long rows,
+                         int k)
+{
+    constexpr int kRows = kRowThreads / kGroup;  // rows per block
+    constexpr int kN = RowVec<T>::kN;
+    __shared__ uint32_t wmax[kRowThreads / 32];
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const int t = threadIdx.x % kGroup;
+    for (long long row0 = static_cast<long long>(blockIdx.x) * kRows; row0 < rows;
+         row0 += static_cast<long long>(gridDim.x) * kRows) {
+        const long long row = row0 + threadIdx.x / kGroup;
+        const bool live = row < rows;
+        const T* xr = x + row * k;
+        int8_t* orow = out + row * k;
+        const int nv = kVec ? k / kN : 0;
+        const uint4* xv = reinterpret_cast<const uint4*>(xr);
+        uint4 v[kRowVecs];
+        uint32_t m = 0u;
+        if (live && kVec) {
+#pragma unroll
+            for (int u = 0; u < kRowVecs; ++u)
+                if (t + u * kGroup < nv) v[u] = xv[t + u * kGroup];
+#pragma unroll
+            for (int u = 0; u < kRowVecs; ++u)
+                if (t + u * kGroup < nv) m = row_absmax<T>(v[u], m);
+            for (int i = t + kRowVecs * kGroup; i < nv; i += kGroup) m = row_absmax<T>(xv[i], m);
+        } else if (live) {
+            for (int i = t; i < k; i += kGroup) m = max(m, __float_as_uint(row_value(xr[i])) & 0x7FFFFFFFu);
+        }
+        m = __reduce_max_sync(0xffffffffu, m);
+        if constexpr (kGroup > 32) {
+            __syncthreads();  // the last row's maxima have been read
+            if ((threadIdx.x & 31) == 0) wmax[threadIdx.x >> 5] = m;
+            __syncthreads();
+            m = wmax[0];
+#pragma unroll
+            for (int w = 1; w < kRowThreads / 32; ++w) m = max(m, wmax[w]);
+        }
+        const float absmax = __uint_as_float(m);
+        const float inv = quant_inv(absmax, 127.f);
+        if (!live) continue;
+        if (t == 0) scale[row] = __fdiv_rn(absmax, 127.f);
+        if constexpr (kVec) {
+#pragma unroll
+            for (int u = 0; u < kRowVecs; ++u)
+                if (t + u * kGroup < nv) row_codes<T>(v[u], inv, orow + (t + u * kGroup) * kN);
+            for (int i = t + kRowVecs * kGroup; i < nv; i += kGroup) row_codes<T>(xv[i], inv, orow + i * kN);
+        } else {
+            for (int i = t; i < k; i += kGroup) orow[i] = static_cast<int8_t>(quant_code(row_value(xr[i]), inv, 127.f));
+        }
+    }
 }
 
 // *scale = absmax / qmax, written over the absmax slot once every quantise

@@ -1,0 +1,412 @@
+// tcg_rows.cu -- host side of the row-scaled and grouped products declared in
+// include/tcgemm.h: checks of arguments, choice of the tile, tensor maps and
+// the launch of rows_kernel (tcg_rows_kernel.cuh).
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <atomic>
+#include <cstring>
+
+#include "../../include/tcgemm.h"
+#include "tcg_host.h"
+#include "tcg_rows_kernel.cuh"
+
+static_assert(TCG_MAX_GROUPS == tcg::kRowsMaxGroups, "groups of the table in shared memory");
+static_assert(TCG_F32 == tcg::kOutF32 && TCG_F16 == tcg::kOutF16 && TCG_BF16 == tcg::kOutBF16, "output types");
+
+namespace {
+
+using namespace tcg;
+
+std::atomic<int> g_rows_tile{0};
+std::atomic<int> g_rows_split{0};
+
+// One product, checked and ready to launch.
+struct RowsCall {
+    const void* pside;      // weights; weight form: the rows' other side (16-bit values or int8 codes)
+    const void* qside;      // rows; weight form: the gradient by the product's result
+    void* out;
+    int out_type;
+    bool bf16;
+    const int32_t* offsets;
+    int groups, rows, P, Q, R;
+    const float *scale_q, *scale_p, *bias_p, *scale_r;
+    int zero_rest;
+    int early;
+};
+
+struct RowsPlan {
+    int bq;     // 16, 32, 64, 128 (kSub = 1) or 256 (kSub = 2)
+    int split;
+};
+
+int ceil_div(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
+
+// Tile and split.  See the measurements in tcg_rows_kernel.cuh.
+RowsPlan choose_plan(const RowsCall& c, bool weight, int kblock, int sms)
+{
+    const int forced = g_rows_tile.load(), forced_split = g_rows_split.load();
+    RowsPlan plan{128, 1};
+    const long long mean = (static_cast<long long>(c.rows) + c.groups - 1) / c.groups;  // rows per group
+    long long wide, tiles;
+    if (weight) {
+        wide = static_cast<long long>(c.groups) * ceil_div(c.P, 256) * ceil_div(c.Q, 256);
+    } else {
+        wide = static_cast<long long>(c.groups) * ceil_div(mean, 256) * ceil_div(c.P, 256);
+    }
+    if (forced) {
+        plan.bq = forced;
+        if (weight && plan.bq < 128) plan.bq = 128;
+    } else if ((weight || mean > 96) && 4 * wide >= 3 * sms) {
+        plan.bq = 256;
+    } else if (!weight) {
+        plan.bq = 16;
+        while (plan.bq < 128 && 4 * plan.bq < 5 * mean) plan.bq *= 2;
+        if (!c.offsets && plan.bq > 16 && plan.bq / 2 >= mean) plan.bq /= 2;
+    }
+    if (plan.bq == 256) return plan;
+    if (weight)
+        tiles = static_cast<long long>(c.groups) * ceil_div(c.P, 128) * ceil_div(c.Q, plan.bq);
+    else
+        tiles = static_cast<long long>(c.groups < c.rows ? c.groups : c.rows) * ceil_div(mean, plan.bq) *
+                ceil_div(c.P, 128);
+    const long long kb = ceil_div(weight ? mean : c.R, kblock);
+    if (forced_split) {
+        plan.split = forced_split;
+    } else {
+        while (plan.split < 8 && tiles * plan.split * 2 <= 2LL * sms && kb >= 8LL * plan.split) plan.split *= 2;
+    }
+    return plan;
+}
+
+template <class C>
+tcg_status launch(const RowsCall& c, int split, int dev, int sms, cudaStream_t st)
+{
+    static std::atomic<bool> smem_set[host::kDevices];
+    auto kern = rows_kernel<C>;
+    constexpr int most = C::smem_bytes(C::kSub == 1 ? 8 : 1, kRowsMaxGroups);
+    static_assert(most <= 232448, "shared memory per CTA");
+    if (!smem_set[dev].load(std::memory_order_acquire)) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+        if (e != cudaSuccess) return host::fail(e);
+        smem_set[dev].store(true, std::memory_order_release);
+    }
+
+    const CUtensorMapDataType t16 = CU_TENSOR_MAP_DATA_TYPE_UINT16, t8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    const CUtensorMapDataType dt = C::kElem == 2 ? t16 : t8;
+    const uint64_t es = C::kElem, P = c.P, Q = c.Q, R = c.R, M = c.rows, G = c.groups;
+    const CUtensorMapSwizzle swz = CU_TENSOR_MAP_SWIZZLE_128B;
+    CUtensorMap mp, mq;
+    tcg_status s;
+    if (C::kConv)
+        s = host::encode_3d(&mp, t8, c.pside, {P, M, 1, P, M * P, 128, C::kBK}, CU_TENSOR_MAP_SWIZZLE_NONE);
+    else if (C::kWeight)
+        s = host::encode_3d(&mp, dt, c.pside, {P, M, 1, P * es, M * P * es, 64, C::kBK}, swz);
+    else if (C::kPMn)
+        s = host::encode_3d(&mp, dt, c.pside, {P, R, G, P * es, R * P * es, 64, C::kBK}, swz);
+    else
+        s = host::encode_3d(&mp, dt, c.pside, {R, P, G, R * es, P * R * es, C::kBK, 128}, swz);
+    if (s != TCG_SUCCESS) return s;
+    if (C::kWeight)
+        s = host::encode_3d(&mq, dt, c.qside, {Q, M, 1, Q * es, M * Q * es, 64, C::kBK}, swz);
+    else
+        s = host::encode_3d(&mq, dt, c.qside, {R, M, 1, R * es, M * R * es, C::kBK, C::kQBox}, swz);
+    if (s != TCG_SUCCESS) return s;
+
+    RowsParams p;
+    std::memset(&p, 0, sizeof p);
+    p.out = c.out;
+    p.offsets = c.offsets;
+    p.scale_q = c.scale_q;
+    p.scale_p = c.scale_p;
+    p.bias_p = c.bias_p;
+    p.scale_r = c.scale_r;
+    p.timeout_ns = host::wait_timeout_ns();
+    p.groups = c.groups;
+    p.rows = c.rows;
+    p.rows_per_group = c.rows / c.groups;
+    p.P = c.P;
+    p.Q = c.Q;
+    p.R = c.R;
+    p.ptiles = ceil_div(c.P, C::kTileP);
+    p.qtiles = ceil_div(c.Q, C::kBQ);
+    p.zero_rest = c.zero_rest;
+    p.out_type = c.out_type;
+    p.bf16 = c.bf16;
+    p.split = split;
+    p.early = c.early;
+    const uint32_t fmt = C::kKind == kKindI8 ? 1u : (c.bf16 ? 1u : 0u);
+    p.idesc = make_idesc(C::kKind == kKindI8 ? 2u : 1u, fmt, fmt, C::kQMn, 128, 0) | (C::kPMn ? 1u << 15 : 0u);
+
+    // an upper bound of the tiles (the bounds of ragged groups are known to the device only)
+    long long qt;
+    if (C::kWeight) {
+        qt = static_cast<long long>(c.groups) * p.qtiles;
+    } else if (c.offsets) {
+        long long parts = c.groups + (c.zero_rest ? 2 : 0);
+        if (parts > c.rows) parts = c.rows;
+        qt = (c.rows + parts * (C::kBQ - 1)) / C::kBQ;
+    } else {
+        qt = static_cast<long long>(c.groups) * ceil_div(p.rows_per_group, C::kBQ);
+    }
+    const long long items = qt * p.ptiles;
+    if (items * split > 0x7fffffffLL) return TCG_ERR_SHAPE;
+    // about square in elements over the tiles in flight
+    const int flight = sms / split;
+    int band = 1;
+    while (band * 2 * band * 2 * static_cast<long long>(C::kBQ) <= static_cast<long long>(flight) * C::kTileP) band *= 2;
+    p.band = band;
+
+    cudaLaunchConfig_t cfg;
+    std::memset(&cfg, 0, sizeof cfg);
+    cudaLaunchAttribute attr[2];
+    std::memset(attr, 0, sizeof attr);
+    const long long grid = C::kSub == 2 && items > sms ? sms : items;
+    cfg.gridDim = dim3(static_cast<unsigned>(grid * split), 1, 1);
+    cfg.blockDim = dim3(C::kThreads, 1, 1);
+    cfg.dynamicSmemBytes = C::smem_bytes(split, c.groups);
+    cfg.stream = st;
+    cfg.attrs = attr;
+    if (split > 1) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs].val.clusterDim.x = static_cast<unsigned>(split);
+        attr[cfg.numAttrs].val.clusterDim.y = 1;
+        attr[cfg.numAttrs].val.clusterDim.z = 1;
+        ++cfg.numAttrs;
+    }
+    if (host::dependent_launch()) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+        ++cfg.numAttrs;
+    }
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, mp, mq, p);
+    return e == cudaSuccess ? TCG_SUCCESS : host::fail(e);
+}
+
+template <int kKind, bool kPMn>
+tcg_status run_rows(const RowsCall& c, cudaStream_t st)
+{
+    int dev, sms;
+    const tcg_status s = host::device(&dev, &sms);
+    if (s != TCG_SUCCESS) return s;
+    const RowsPlan plan = choose_plan(c, false, kKind == kKindF16 ? 64 : 128, sms);
+    switch (plan.bq) {
+    case 16: return launch<RowsTraits<kKind, kPMn, false, false, 1, 16, 5>>(c, plan.split, dev, sms, st);
+    case 32: return launch<RowsTraits<kKind, kPMn, false, false, 1, 32, 5>>(c, plan.split, dev, sms, st);
+    case 64: return launch<RowsTraits<kKind, kPMn, false, false, 1, 64, 4>>(c, plan.split, dev, sms, st);
+    case 128: return launch<RowsTraits<kKind, kPMn, false, false, 1, 128, 3>>(c, plan.split, dev, sms, st);
+    default: return launch<RowsTraits<kKind, kPMn, false, false, 2, 256, 3>>(c, 1, dev, sms, st);
+    }
+}
+
+template <bool kConv>
+tcg_status run_weight(const RowsCall& c, cudaStream_t st)
+{
+    int dev, sms;
+    const tcg_status s = host::device(&dev, &sms);
+    if (s != TCG_SUCCESS) return s;
+    const RowsPlan plan = choose_plan(c, true, 64, sms);
+    if (plan.bq == 256) return launch<RowsTraits<kKindF16, true, true, kConv, 2, 256, 3>>(c, 1, dev, sms, st);
+    return launch<RowsTraits<kKindF16, true, true, kConv, 1, 128, 3>>(c, plan.split, dev, sms, st);
+}
+
+bool is_type(tcg_dtype t) { return t == TCG_F32 || t == TCG_F16 || t == TCG_BF16; }
+bool misaligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) % n) != 0; }
+unsigned size_of(tcg_dtype t) { return t == TCG_F32 ? 4u : 2u; }
+size_t round256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
+
+// Checks shared by every form; *done: there is no output.
+tcg_status check(int M, int N, int K, int groups, const int32_t* offsets, long long out_elems, bool* done)
+{
+    *done = false;
+    if (M < 0 || N < 0 || K < 0 || groups < 0) return TCG_ERR_SHAPE;
+    if (out_elems == 0) {
+        *done = true;
+        return TCG_SUCCESS;
+    }
+    if (groups == 0 || groups > TCG_MAX_GROUPS) return TCG_ERR_SHAPE;
+    if (!offsets && M % groups != 0) return TCG_ERR_SHAPE;
+    if (misaligned(offsets, 4)) return TCG_ERR_ALIGN;
+    return TCG_SUCCESS;
+}
+
+tcg_status gemm_s8(const int8_t* A, const int8_t* B, void* C, tcg_dtype c_type, const int32_t* offsets, int groups,
+                   int M, int N, int K, const float* scale_a, const float* scale_b, const float* bias, int zero_rest,
+                   int early, cudaStream_t st)
+{
+    if (!A || !B || !C || !scale_a || !scale_b) return TCG_ERR_ARG;
+    if (K == 0 || K % 16 != 0) return TCG_ERR_SHAPE;
+    if (misaligned(A, 16) || misaligned(B, 16) || misaligned(C, size_of(c_type)) || misaligned(scale_a, 4) ||
+        misaligned(scale_b, 4) || misaligned(bias, 4))
+        return TCG_ERR_ALIGN;
+    RowsCall c;
+    std::memset(&c, 0, sizeof c);
+    c.pside = B;
+    c.qside = A;
+    c.out = C;
+    c.out_type = c_type;
+    c.offsets = offsets;
+    c.groups = groups;
+    c.rows = M;
+    c.P = N;
+    c.R = K;
+    c.scale_q = scale_a;
+    c.scale_p = scale_b;
+    c.bias_p = bias;
+    c.zero_rest = zero_rest;
+    c.early = early && host::dependent_launch();
+    return run_rows<kKindI8, false>(c, st);
+}
+
+}  // namespace
+
+namespace tcg {
+namespace host {
+
+tcg_status take_rows_error(unsigned long long* word)
+{
+    cudaError_t e = cudaMemcpyFromSymbol(word, tcg::g_tcg_error_word, sizeof *word);
+    const unsigned long long zero = 0;
+    if (e == cudaSuccess && *word != 0) e = cudaMemcpyToSymbol(tcg::g_tcg_error_word, &zero, sizeof zero);
+    return e == cudaSuccess ? TCG_SUCCESS : fail(e);
+}
+
+}  // namespace host
+}  // namespace tcg
+
+extern "C" {
+
+tcg_status tcg_gemm_s8_grouped(const int8_t* A, const int8_t* B, void* C, tcg_dtype c_type, const int32_t* offsets,
+                               int groups, int M, int N, int K, const float* scale_a, const float* scale_b,
+                               const float* bias, int zero_rest, void* stream)
+{
+    if (!is_type(c_type)) return TCG_ERR_ARG;
+    bool done;
+    const tcg_status s = check(M, N, K, groups, offsets, static_cast<long long>(M) * N, &done);
+    if (s != TCG_SUCCESS || done) return s;
+    return gemm_s8(A, B, C, c_type, offsets, groups, M, N, K, scale_a, scale_b, bias, zero_rest, 0,
+                   static_cast<cudaStream_t>(stream));
+}
+
+tcg_status tcg_gemm_s8_scaled(const int8_t* A, const int8_t* B, void* C, tcg_dtype c_type, int M, int N, int K,
+                              int batches, const float* scale_a, const float* scale_b, const float* bias,
+                              void* stream)
+{
+    if (M < 0 || batches < 0) return TCG_ERR_SHAPE;
+    const long long rows = static_cast<long long>(M) * batches;
+    if (rows > 0x7fffffffLL) return TCG_ERR_SHAPE;
+    return tcg_gemm_s8_grouped(A, B, C, c_type, nullptr, batches, static_cast<int>(rows), N, K, scale_a, scale_b, bias,
+                               0, stream);
+}
+
+size_t tcg_linear_s8_workspace_size(int M, int K)
+{
+    if (M <= 0 || K <= 0) return 0;
+    return round256(static_cast<size_t>(M) * K) + round256(static_cast<size_t>(M) * sizeof(float));
+}
+
+tcg_status tcg_linear_s8_grouped(const void* x, tcg_dtype x_type, const int8_t* B, void* C, tcg_dtype c_type,
+                                 const int32_t* offsets, int groups, int M, int N, int K, const float* scale_b,
+                                 const float* bias, int zero_rest, void* workspace, size_t workspace_bytes,
+                                 void* stream)
+{
+    if (!is_type(x_type) || !is_type(c_type)) return TCG_ERR_ARG;
+    bool done;
+    tcg_status s = check(M, N, K, groups, offsets, static_cast<long long>(M) * N, &done);
+    if (s != TCG_SUCCESS || done) return s;
+    // everything is checked before the first launch
+    if (!x || !B || !C || !scale_b || !workspace) return TCG_ERR_ARG;
+    if (K == 0 || K % 16 != 0) return TCG_ERR_SHAPE;
+    if (workspace_bytes < tcg_linear_s8_workspace_size(M, K)) return TCG_ERR_WORKSPACE;
+    if (misaligned(workspace, 256) || misaligned(x, size_of(x_type)) || misaligned(B, 16) ||
+        misaligned(C, size_of(c_type)) || misaligned(scale_b, 4) || misaligned(bias, 4))
+        return TCG_ERR_ALIGN;
+    int8_t* codes = static_cast<int8_t*>(workspace);
+    float* scale = reinterpret_cast<float*>(codes + round256(static_cast<size_t>(M) * K));
+    s = tcg_quantize_rows_s8(x, x_type, codes, scale, M, K, stream);
+    if (s != TCG_SUCCESS) return s;
+    return gemm_s8(codes, B, C, c_type, offsets, groups, M, N, K, scale, scale_b, bias, zero_rest, 1,
+                   static_cast<cudaStream_t>(stream));
+}
+
+tcg_status tcg_linear_s8(const void* x, tcg_dtype x_type, const int8_t* B, void* C, tcg_dtype c_type, int M, int N,
+                         int K, const float* scale_b, const float* bias, void* workspace, size_t workspace_bytes,
+                         void* stream)
+{
+    return tcg_linear_s8_grouped(x, x_type, B, C, c_type, nullptr, 1, M, N, K, scale_b, bias, 0, workspace,
+                                 workspace_bytes, stream);
+}
+
+tcg_status tcg_gemm_16_grouped(const void* A, const void* B, tcg_dtype type, void* C, tcg_dtype c_type,
+                               const int32_t* offsets, int groups, int M, int N, int K, tcg_b_layout b_layout,
+                               int zero_rest, void* stream)
+{
+    if ((type != TCG_F16 && type != TCG_BF16) || !is_type(c_type)) return TCG_ERR_ARG;
+    if (b_layout != TCG_B_KN && b_layout != TCG_B_NK) return TCG_ERR_ARG;
+    bool done;
+    const tcg_status s = check(M, N, K, groups, offsets, static_cast<long long>(M) * N, &done);
+    if (s != TCG_SUCCESS || done) return s;
+    if (!A || !B || !C) return TCG_ERR_ARG;
+    if (K == 0 || K % 8 != 0 || (b_layout == TCG_B_KN && N % 8 != 0)) return TCG_ERR_SHAPE;
+    if (misaligned(A, 16) || misaligned(B, 16) || misaligned(C, size_of(c_type))) return TCG_ERR_ALIGN;
+    RowsCall c;
+    std::memset(&c, 0, sizeof c);
+    c.pside = B;
+    c.qside = A;
+    c.out = C;
+    c.out_type = c_type;
+    c.bf16 = type == TCG_BF16;
+    c.offsets = offsets;
+    c.groups = groups;
+    c.rows = M;
+    c.P = N;
+    c.R = K;
+    c.zero_rest = zero_rest;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return b_layout == TCG_B_NK ? run_rows<kKindF16, false>(c, st) : run_rows<kKindF16, true>(c, st);
+}
+
+tcg_status tcg_gemm_16_grouped_wgrad(const void* dC, const void* A, const float* scale_a, tcg_dtype type, void* dB,
+                                     tcg_dtype b_type, const int32_t* offsets, int groups, int M, int N, int K,
+                                     void* stream)
+{
+    if ((type != TCG_F16 && type != TCG_BF16) || !is_type(b_type)) return TCG_ERR_ARG;
+    bool done;
+    const long long weights = static_cast<long long>(groups < 0 ? 0 : groups) * N;
+    const tcg_status s = check(M, N, K, groups, offsets, K > 0 ? weights : 0, &done);
+    if (s != TCG_SUCCESS || done) return s;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (!dB) return TCG_ERR_ARG;
+    if (N % 8 != 0 || K % (scale_a ? 16 : 8) != 0) return TCG_ERR_SHAPE;
+    if (misaligned(dB, size_of(b_type)) || misaligned(scale_a, 4)) return TCG_ERR_ALIGN;
+    if (M == 0) {  // no rows at all: every gradient is zero
+        const cudaError_t e = cudaMemsetAsync(dB, 0, static_cast<size_t>(weights) * K * size_of(b_type), st);
+        return e == cudaSuccess ? TCG_SUCCESS : host::fail(e);
+    }
+    if (!dC || !A) return TCG_ERR_ARG;
+    if (misaligned(dC, 16) || misaligned(A, 16)) return TCG_ERR_ALIGN;
+    RowsCall c;
+    std::memset(&c, 0, sizeof c);
+    c.pside = A;
+    c.qside = dC;
+    c.out = dB;
+    c.out_type = b_type;
+    c.bf16 = type == TCG_BF16;
+    c.offsets = offsets;
+    c.groups = groups;
+    c.rows = M;
+    c.P = K;
+    c.Q = N;
+    c.scale_r = scale_a;
+    return scale_a ? run_weight<true>(c, st) : run_weight<false>(c, st);
+}
+
+void tcg_set_rows_tile(int rows, int split)
+{
+    const bool tile = rows == 16 || rows == 32 || rows == 64 || rows == 128 || rows == 256;
+    const bool parts = split == 1 || split == 2 || split == 4 || split == 8;
+    g_rows_tile.store(tile ? rows : 0);
+    g_rows_split.store(parts ? split : 0);
+}
+
+}  // extern "C"

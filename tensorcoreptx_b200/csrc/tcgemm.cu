@@ -17,6 +17,7 @@
 
 #include "../../include/tcgemm.h"
 #include "tcg_gemm_kernel.cuh"
+#include "tcg_host.h"
 #include "tcg_quant.cuh"
 
 namespace {
@@ -146,9 +147,17 @@ tcg_status encode_3d_uncached(CUtensorMap* map, CUtensorMapDataType dt, const vo
     cuuint64_t strides[2] = {s1, s2};
     cuuint32_t box[3] = {box0, box1, 1};
     cuuint32_t estr[3] = {1, 1, 1};
-    CUresult r = g_encode(map, dt, 3, const_cast<void*>(base), dims, strides, box, estr,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
-                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const auto encode = [&]() {
+        return g_encode(map, dt, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        swz, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = encode();
+    if (r == CUDA_ERROR_INVALID_CONTEXT) {
+        // a thread on which the runtime has not bound the device's context yet
+        // (an autograd worker, say): the encoder is a driver call and needs it
+        int dev = 0;
+        if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = encode();
+    }
     if (r != CUDA_SUCCESS) {
         t_last_cuda_error = static_cast<int>(r);
         return TCG_ERR_CUDA;
@@ -588,6 +597,35 @@ tcg_status launch_unpack(const int8_t* in0, int8_t* out0, size_t n0, const int8_
 
 }  // namespace
 
+// ---- shared with the library's other translation units (tcg_host.h) -------
+
+namespace tcg {
+namespace host {
+
+tcg_status fail(cudaError_t e) { return cuda_fail(e); }
+
+tcg_status device(int* id, int* sms)
+{
+    DeviceState* d;
+    const tcg_status s = device_state(&d);
+    if (s != TCG_SUCCESS) return s;
+    *id = static_cast<int>(d - g_dev);
+    *sms = d->sms;
+    return resolve_encode();
+}
+
+tcg_status encode_3d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, const Box3& b,
+                     CUtensorMapSwizzle swz)
+{
+    return encode_3d_uncached(map, dt, base, b.d0, b.d1, b.d2, b.s1, b.s2, b.box0, b.box1, swz);
+}
+
+bool dependent_launch() { return pdl_enabled(); }
+unsigned long long wait_timeout_ns() { return g_timeout_ns.load(); }
+
+}  // namespace host
+}  // namespace tcg
+
 extern "C" {
 
 tcg_status tcg_gemm_f16(const void* A, const void* B, float* C, int M, int N, int K, int batches, tcg_acc acc,
@@ -858,6 +896,78 @@ tcg_status tcg_quantize_absmax_s4(const float* src, int8_t* dst_packed, int rows
 
 }  // extern "C"
 
+// ---- quantisation with a scale per row ------------------------------------
+
+namespace {
+
+template <class T, int kGroup, bool kVec>
+tcg_status launch_quantize_rows(const void* src, int8_t* dst, float* scale, long long rows, int k, int sms,
+                                cudaStream_t st)
+{
+    constexpr int per_block = kRowThreads / kGroup;
+    long long blocks = (rows + per_block - 1) / per_block;
+    const long long cap = static_cast<long long>(sms) * 32;
+    if (blocks > cap) blocks = cap;
+    cudaLaunchConfig_t cfg;
+    std::memset(&cfg, 0, sizeof cfg);
+    cudaLaunchAttribute attr[1];
+    std::memset(attr, 0, sizeof attr);
+    cfg.gridDim = dim3(static_cast<unsigned>(blocks), 1, 1);
+    cfg.blockDim = dim3(kRowThreads, 1, 1);
+    cfg.stream = st;
+    cfg.attrs = attr;
+    if (pdl_enabled()) {
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.numAttrs = 1;
+    }
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, quantize_rows_kernel<T, kGroup, kVec>, static_cast<const T*>(src),
+                                             dst, scale, rows, k);
+    return e == cudaSuccess ? TCG_SUCCESS : cuda_fail(e);
+}
+
+// A warp per row while the row fits its registers (one pass, no block
+// barrier) and there are rows enough for every SM; a block per row otherwise.
+template <class T>
+tcg_status quantize_rows(const void* src, int8_t* dst, float* scale, long long rows, int k, int sms, cudaStream_t st)
+{
+    constexpr int kN = 16 / sizeof(T);
+    const bool vec = k % kN == 0 && aligned16(src) && (reinterpret_cast<uintptr_t>(dst) % kN) == 0;
+    if (!vec) return launch_quantize_rows<T, kRowThreads, false>(src, dst, scale, rows, k, sms, st);
+    if (k <= 32 * kRowVecs * kN && rows >= 4LL * sms)
+        return launch_quantize_rows<T, 32, true>(src, dst, scale, rows, k, sms, st);
+    return launch_quantize_rows<T, kRowThreads, true>(src, dst, scale, rows, k, sms, st);
+}
+
+}  // namespace
+
+extern "C" {
+
+tcg_status tcg_quantize_rows_s8(const void* src, tcg_dtype type, int8_t* dst, float* scale, long long rows, int k,
+                                void* stream)
+{
+    if (type != TCG_F32 && type != TCG_F16 && type != TCG_BF16) return TCG_ERR_ARG;
+    if (rows < 0 || k < 0) return TCG_ERR_SHAPE;
+    if (rows == 0) return TCG_SUCCESS;
+    if (!scale) return TCG_ERR_ARG;
+    if (reinterpret_cast<uintptr_t>(scale) & 3u) return TCG_ERR_ALIGN;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (k == 0) {  // no values: scales of zero
+        const cudaError_t e = cudaMemsetAsync(scale, 0, static_cast<size_t>(rows) * sizeof(float), st);
+        return e == cudaSuccess ? TCG_SUCCESS : cuda_fail(e);
+    }
+    if (!src || !dst) return TCG_ERR_ARG;
+    if (reinterpret_cast<uintptr_t>(src) % (type == TCG_F32 ? 4u : 2u)) return TCG_ERR_ALIGN;
+    DeviceState* dev;
+    const tcg_status s = device_state(&dev);
+    if (s != TCG_SUCCESS) return s;
+    if (type == TCG_F32) return quantize_rows<float>(src, dst, scale, rows, k, dev->sms, st);
+    if (type == TCG_F16) return quantize_rows<__half>(src, dst, scale, rows, k, dev->sms, st);
+    return quantize_rows<__nv_bfloat16>(src, dst, scale, rows, k, dev->sms, st);
+}
+
+}  // extern "C"
+
 // ---- int4 GEMM without allocation: scratch in a fixed device array -------
 //
 // For callers that may not allocate device memory (see tcgemm.h).  Host code
@@ -937,12 +1047,15 @@ tcg_status tcg_check_device_error(void* stream, uint64_t* word)
     unsigned long long w = 0;
     e = cudaMemcpyFromSymbol(&w, tcg::g_tcg_error_word, sizeof w);
     if (e != cudaSuccess) return cuda_fail(e);
-    if (word) *word = w;
-    if (w == 0) return TCG_SUCCESS;
     const unsigned long long zero = 0;
-    e = cudaMemcpyToSymbol(tcg::g_tcg_error_word, &zero, sizeof zero);
-    if (e != cudaSuccess) return cuda_fail(e);
-    return TCG_ERR_TIMEOUT;
+    if (w != 0 && (e = cudaMemcpyToSymbol(tcg::g_tcg_error_word, &zero, sizeof zero)) != cudaSuccess)
+        return cuda_fail(e);
+    unsigned long long rows = 0;
+    const tcg_status s = tcg::host::take_rows_error(&rows);
+    if (s != TCG_SUCCESS) return s;
+    if (w == 0) w = rows;
+    if (word) *word = w;
+    return w == 0 ? TCG_SUCCESS : TCG_ERR_TIMEOUT;
 }
 
 tcg_status tcg_ipc_handle(const void* ptr, void* handle, size_t* offset)
