@@ -84,8 +84,7 @@ tcg_status launch(const RowsCall& c, int split, int dev, int sms, cudaStream_t s
 {
     static std::atomic<bool> smem_set[host::kDevices];
     auto kern = rows_kernel<C>;
-    constexpr int most = C::smem_bytes(C::kSub == 1 ? 8 : 1, kRowsMaxGroups);
-    static_assert(most <= 232448, "shared memory per CTA");
+    constexpr int most = 232448;  // shared memory per CTA
     if (!smem_set[dev].load(std::memory_order_acquire)) {
         const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
         if (e != cudaSuccess) return host::fail(e);
@@ -129,42 +128,52 @@ tcg_status launch(const RowsCall& c, int split, int dev, int sms, cudaStream_t s
     p.Q = c.Q;
     p.R = c.R;
     p.ptiles = ceil_div(c.P, C::kTileP);
-    p.qtiles = ceil_div(c.Q, C::kBQ);
+    p.qtiles = ceil_div(C::kWeight ? c.Q : p.rows_per_group, C::kBQ);
     p.zero_rest = c.zero_rest;
     p.out_type = c.out_type;
     p.bf16 = c.bf16;
-    p.split = split;
+    while ((1 << p.split_log2) < split) ++p.split_log2;
     p.early = c.early;
+    const int table = c.offsets ? c.groups : 0;
     const uint32_t fmt = C::kKind == kKindI8 ? 1u : (c.bf16 ? 1u : 0u);
     p.idesc = make_idesc(C::kKind == kKindI8 ? 2u : 1u, fmt, fmt, C::kQMn, 128, 0) | (C::kPMn ? 1u << 15 : 0u);
 
     // an upper bound of the tiles (the bounds of ragged groups are known to the device only)
-    long long qt;
-    if (C::kWeight) {
-        qt = static_cast<long long>(c.groups) * p.qtiles;
-    } else if (c.offsets) {
+    long long qt = static_cast<long long>(c.groups) * p.qtiles;
+    if (!C::kWeight && c.offsets) {
         long long parts = c.groups + (c.zero_rest ? 2 : 0);
         if (parts > c.rows) parts = c.rows;
         qt = (c.rows + parts * (C::kBQ - 1)) / C::kBQ;
-    } else {
-        qt = static_cast<long long>(c.groups) * ceil_div(p.rows_per_group, C::kBQ);
     }
     const long long items = qt * p.ptiles;
-    if (items * split > 0x7fffffffLL) return TCG_ERR_SHAPE;
-    // about square in elements over the tiles in flight
-    const int flight = sms / split;
-    int band = 1;
-    while (band * 2 * band * 2 * static_cast<long long>(C::kBQ) <= static_cast<long long>(flight) * C::kTileP) band *= 2;
-    p.band = band;
+    if (items > 0x7fffffffLL / 8 || p.ptiles > 65535) return TCG_ERR_SHAPE;
+    // bands about square in elements over the tiles in flight
+    while ((4LL << (2 * p.band_log2)) * C::kBQ <= static_cast<long long>(sms) * C::kTileP) ++p.band_log2;
+    p.per_band_inv = div_inverse(static_cast<uint32_t>(p.ptiles) << p.band_log2);
+    p.ptiles_inv = div_inverse(p.ptiles);
+    p.per_group_inv = div_inverse(static_cast<uint32_t>(C::kWeight ? p.ptiles * p.qtiles : p.qtiles));
 
     cudaLaunchConfig_t cfg;
     std::memset(&cfg, 0, sizeof cfg);
     cudaLaunchAttribute attr[2];
     std::memset(attr, 0, sizeof attr);
-    const long long grid = C::kSub == 2 && items > sms ? sms : items;
-    cfg.gridDim = dim3(static_cast<unsigned>(grid * split), 1, 1);
+    if (C::kSub == 2)
+        cfg.gridDim = dim3(static_cast<unsigned>(items > sms ? sms : items), 1, 1);
+    else if (C::kWeight)
+        cfg.gridDim = dim3(static_cast<unsigned>(p.qtiles * split), p.ptiles, c.groups);
+    else
+        cfg.gridDim = dim3(static_cast<unsigned>(qt * split), p.ptiles, 1);
     cfg.blockDim = dim3(C::kThreads, 1, 1);
-    cfg.dynamicSmemBytes = C::smem_bytes(split, c.groups);
+    // Ring depth: all of shared memory for one CTA per SM; half of it, so that
+    // one CTA's start and end overlap another's loads, where there are more
+    // CTAs than SMs (kSub = 1).
+    const int room = C::kSub == 1 && items * split > sms && 2 * C::smem_bytes(2, split, table) <= most - 2048
+                         ? (most - 2048) / 2
+                         : most;
+    int stages = (room - C::smem_bytes(0, split, table)) / C::kStageBytes;
+    if (stages > C::kMaxStages) stages = C::kMaxStages;
+    p.stages = stages;
+    cfg.dynamicSmemBytes = C::smem_bytes(stages, split, table);
     cfg.stream = st;
     cfg.attrs = attr;
     if (split > 1) {
@@ -191,11 +200,11 @@ tcg_status run_rows(const RowsCall& c, cudaStream_t st)
     if (s != TCG_SUCCESS) return s;
     const RowsPlan plan = choose_plan(c, false, kKind == kKindF16 ? 64 : 128, sms);
     switch (plan.bq) {
-    case 16: return launch<RowsTraits<kKind, kPMn, false, false, 1, 16, 5>>(c, plan.split, dev, sms, st);
-    case 32: return launch<RowsTraits<kKind, kPMn, false, false, 1, 32, 5>>(c, plan.split, dev, sms, st);
-    case 64: return launch<RowsTraits<kKind, kPMn, false, false, 1, 64, 4>>(c, plan.split, dev, sms, st);
-    case 128: return launch<RowsTraits<kKind, kPMn, false, false, 1, 128, 3>>(c, plan.split, dev, sms, st);
-    default: return launch<RowsTraits<kKind, kPMn, false, false, 2, 256, 3>>(c, 1, dev, sms, st);
+    case 16: return launch<RowsTraits<kKind, kPMn, false, false, 1, 16>>(c, plan.split, dev, sms, st);
+    case 32: return launch<RowsTraits<kKind, kPMn, false, false, 1, 32>>(c, plan.split, dev, sms, st);
+    case 64: return launch<RowsTraits<kKind, kPMn, false, false, 1, 64>>(c, plan.split, dev, sms, st);
+    case 128: return launch<RowsTraits<kKind, kPMn, false, false, 1, 128>>(c, plan.split, dev, sms, st);
+    default: return launch<RowsTraits<kKind, kPMn, false, false, 2, 256>>(c, 1, dev, sms, st);
     }
 }
 
@@ -206,8 +215,8 @@ tcg_status run_weight(const RowsCall& c, cudaStream_t st)
     const tcg_status s = host::device(&dev, &sms);
     if (s != TCG_SUCCESS) return s;
     const RowsPlan plan = choose_plan(c, true, 64, sms);
-    if (plan.bq == 256) return launch<RowsTraits<kKindF16, true, true, kConv, 2, 256, 3>>(c, 1, dev, sms, st);
-    return launch<RowsTraits<kKindF16, true, true, kConv, 1, 128, 3>>(c, plan.split, dev, sms, st);
+    if (plan.bq == 256) return launch<RowsTraits<kKindF16, true, true, kConv, 2, 256>>(c, 1, dev, sms, st);
+    return launch<RowsTraits<kKindF16, true, true, kConv, 1, 128>>(c, plan.split, dev, sms, st);
 }
 
 bool is_type(tcg_dtype t) { return t == TCG_F32 || t == TCG_F16 || t == TCG_BF16; }

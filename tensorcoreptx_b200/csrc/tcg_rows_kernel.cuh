@@ -56,20 +56,22 @@ struct RowsParams {
     int groups, rows, rows_per_group;
     int P, Q, R;              // features out; weight form: the other features; rows form: length of the sum
     int ptiles, qtiles;       // tiles along P; weight form: along Q
-    int band;                 // tiles along q per rasterisation band
+    int band_log2;            // kSub = 2: tiles along q per rasterisation band
+    uint32_t per_band_inv, ptiles_inv, per_group_inv;  // div_by: band * ptiles, ptiles, tiles per group
     int zero_rest;            // rows form: write zeros into rows outside every group
     int out_type;
     int bf16;                 // 16-bit operands are bf16 (kConv: type of the widened codes)
-    int split;                // CTAs per tile (kSub = 1)
+    int split_log2;           // kSub = 1: 1, 2, 4 or 8 CTAs per tile
+    int stages;               // ring depth
     int early;                // the M-side operand and the offsets predate the kernel this one follows
     uint32_t idesc;           // instruction descriptor without N
 };
 
-template <int kKind_, bool kPMn_, bool kQMn_, bool kConv_, int kSub_, int kBQ_, int kStages_>
+template <int kKind_, bool kPMn_, bool kQMn_, bool kConv_, int kSub_, int kBQ_>
 struct RowsTraits {
     static constexpr int kKind = kKind_;
     static constexpr bool kPMn = kPMn_, kQMn = kQMn_, kConv = kConv_;
-    static constexpr int kSub = kSub_, kBQ = kBQ_, kStages = kStages_;
+    static constexpr int kSub = kSub_, kBQ = kBQ_;
     static constexpr bool kWeight = kQMn;               // weight form: the sum runs over a group's rows
     static constexpr int kElem = kKind == kKindF16 ? 2 : 1;
     static constexpr int kBK = 128 / kElem;             // length of the sum per ring stage
@@ -86,18 +88,19 @@ struct RowsTraits {
     static constexpr int kThreads = 192 + 32 * kConvWarps;
     static constexpr int kTmemCols = kSub * kBQ < 32 ? 32 : kSub * kBQ;
     static constexpr int kRedBytes = kBQ * 512;         // split: 128 x kBQ partial sums
-    static constexpr int kBarBytes = 256;
-    static constexpr int kRingBytes = kStages * kStageBytes;
+    static constexpr int kMaxStages = 12;
+    static constexpr int kBarBytes = 384;
+    static constexpr int kScaleBytes = 512;             // split: scales of the rows a CTA finishes
     static_assert(!kConv || (kPMn && kQMn && kKind == kKindF16), "converted operand: weight form only");
     static_assert(!kQMn || kKind == kKindF16, "weight form: 16-bit operands");
     static_assert(!kPMn || kKind == kKindF16, "MN-major features: 16-bit operands");
     static_assert(!kQMn || kBQ % 64 == 0, "whole 64-column atoms");
-    static_assert(8 * (3 * kStages + 5) + 16 <= kBarBytes, "barrier area");
+    static_assert(8 * (3 * kMaxStages + 5) + 16 <= kBarBytes, "barrier area");
     static_assert((kTmemCols & (kTmemCols - 1)) == 0 && kTmemCols <= 512, "TMEM allocation");
-    // dynamic shared memory of a launch with `groups` ragged groups
-    static constexpr int smem_bytes(int split, int groups_in_table)
+    // dynamic shared memory of a launch with a table of `groups` groups
+    static constexpr int smem_bytes(int stages, int split, int groups)
     {
-        return 1024 + kRingBytes + (split > 1 ? kRedBytes : 0) + kBarBytes + 8 * (groups_in_table + 3);
+        return 1024 + stages * kStageBytes + (split > 1 ? kRedBytes + kScaleBytes : 0) + kBarBytes + 8 * (groups + 3);
     }
 };
 
@@ -143,37 +146,36 @@ __device__ __forceinline__ void rows_table(const RowsParams& p, int bq, int* bou
     }
 }
 
-template <class C>
-__device__ __forceinline__ int rows_total(const RowsParams& p, const int* cum)
+// a / d for 0 <= a < 2^31 with inv = div_inverse(d): the product with the
+// rounded-up reciprocal is at most one too large.
+__host__ __device__ constexpr uint32_t div_inverse(uint32_t d)
 {
-    if (C::kWeight) return p.groups * p.ptiles * p.qtiles;
-    const int tiles =
-        p.offsets ? cum[p.groups + 2] : p.groups * ((p.rows_per_group + C::kBQ - 1) / C::kBQ);
-    return tiles * p.ptiles;
+    return d <= 1 ? 0u : static_cast<uint32_t>((0x100000000ull + d - 1) / d);
+}
+__device__ __forceinline__ int div_by(int a, int d, uint32_t inv)
+{
+    if (d <= 1) return a;
+    int q = static_cast<int>(__umulhi(static_cast<uint32_t>(a), inv));
+    if (q * d > a) --q;
+    return q;
 }
 
-// Work item -> tile.  Items walk a band of `band` q-tiles for all of P before
-// the next band, so the tiles in flight share both operands in L2.
+// Tiles along q (weight form: of every group together).
 template <class C>
-__device__ __forceinline__ RowsItem rows_item(const RowsParams& p, int item, int total, const int* bound,
+__device__ __forceinline__ int rows_qtiles(const RowsParams& p, const int* cum)
+{
+    if (C::kWeight) return p.groups * p.qtiles;
+    return p.offsets ? cum[p.groups + 2] : p.groups * p.qtiles;
+}
+
+// The tile at p-tile pt and q-tile tq (weight form: tq of group e).
+template <class C>
+__device__ __forceinline__ RowsItem rows_tile(const RowsParams& p, int pt, int tq, int e, const int* bound,
                                               const int* cum)
 {
     RowsItem w;
     w.zero = false;
-    int e = 0;
-    if (C::kWeight) {
-        const int per = p.ptiles * p.qtiles;
-        e = item / per;
-        item -= e * per;
-        total = per;
-    }
-    const int tall = total / p.ptiles;
-    const int per_band = p.band * p.ptiles;
-    const int b = item / per_band;
-    const int r = item - b * per_band;
-    const int width = min(p.band, tall - b * p.band);
-    const int tq = b * p.band + r % width;
-    w.p0 = (r / width) * C::kTileP;
+    w.p0 = pt * C::kTileP;
     if (C::kWeight) {
         w.e = e;
         w.q0 = tq * C::kBQ;
@@ -198,14 +200,42 @@ __device__ __forceinline__ RowsItem rows_item(const RowsParams& p, int item, int
         w.row0 = bound[lo] + (tq - cum[lo]) * C::kBQ;
         w.rend = bound[lo + 1];
     } else {
-        const int per = (p.rows_per_group + C::kBQ - 1) / C::kBQ;
-        w.e = tq / per;
-        w.row0 = w.e * p.rows_per_group + (tq - w.e * per) * C::kBQ;
+        w.e = div_by(tq, p.qtiles, p.per_group_inv);
+        w.row0 = w.e * p.rows_per_group + (tq - w.e * p.qtiles) * C::kBQ;
         w.rend = (w.e + 1) * p.rows_per_group;
     }
     w.cnt = min(C::kBQ, w.rend - w.row0);
     w.nkb = w.zero ? 0 : (p.R + C::kBK - 1) / C::kBK;
     return w;
+}
+
+// Work item of a persistent CTA (kSub = 2) -> tile.  Items walk a band of
+// 2^band_log2 q-tiles for all of P before the next band, so the tiles in
+// flight share both operands in L2; a last, narrower band goes row by row.
+template <class C>
+__device__ __forceinline__ RowsItem rows_item(const RowsParams& p, int item, int qtiles, const int* bound,
+                                              const int* cum)
+{
+    int e = 0;
+    if (C::kWeight) {
+        const int per = p.ptiles * p.qtiles;
+        e = div_by(item, per, p.per_group_inv);
+        item -= e * per;
+        qtiles = p.qtiles;
+    }
+    const int per_band = p.ptiles << p.band_log2;
+    const int b = div_by(item, per_band, p.per_band_inv);
+    const int r = item - b * per_band;
+    int tq = b << p.band_log2, pt;
+    if (tq + (1 << p.band_log2) <= qtiles) {
+        tq += r & ((1 << p.band_log2) - 1);
+        pt = r >> p.band_log2;
+    } else {
+        const int j = div_by(r, p.ptiles, p.ptiles_inv);
+        tq += j;
+        pt = r - j * p.ptiles;
+    }
+    return rows_tile<C>(p, pt, tq, e, bound, cum);
 }
 
 // 32 accumulator words of one lane (one feature, columns c .. c + 31 of the
@@ -304,6 +334,82 @@ __device__ __forceinline__ void conv_write(uint8_t* p_area, int ct, int valid, c
     }
 }
 
+// Split sums.  Columns c .. c + n - 1 of this CTA's part (one lane = feature
+// f) to the CTAs that finish them: CTA d finishes columns d * kBQ / S onwards.
+// There the parts lie as [source rank][group of V columns][feature][V], V = 4
+// (2 for two columns a CTA): one 16-byte store per four columns and lane, and
+// a warp's stores are contiguous.
+template <class C>
+__device__ __forceinline__ void push_part(const uint32_t (&v)[32], uint32_t* red, int rank, int split_log2, int c,
+                                          int n, int f)
+{
+    const int per = C::kBQ >> split_log2;
+    const int per_log2 = 31 - __clz(per);
+#pragma unroll
+    for (int j = 0; j < (C::kBQ < 32 ? C::kBQ : 32); j += 4) {
+        if (j >= n) break;
+        const int d = (c + j) >> per_log2, cl = (c + j) & (per - 1);
+        if (per >= 4) {
+            const uint32_t at = smem_u32(red + (rank * per + cl) * 128 + f * 4);
+            st_cluster_v4(mapa_shared(at, d), v[j], v[j + 1], v[j + 2], v[j + 3]);
+        } else {
+            const uint32_t at = smem_u32(red + rank * 256 + f * 2);
+            st_cluster_v2(mapa_shared(at, d), v[j], v[j + 1]);
+            st_cluster_v2(mapa_shared(at, d + 1), v[j + 2], v[j + 3]);
+        }
+    }
+}
+
+// This CTA's columns of the tile: the parts added in rank order, scaled, and
+// stored; one thread per feature, V columns at a time.
+template <class C, int V, class T>
+__device__ __forceinline__ void finish_parts(const RowsParams& p, const RowsItem& w, const uint32_t* red,
+                                             const float* scale, int rank, int t, float sp, float bias)
+{
+    const int S = 1 << p.split_log2;
+    const int per = C::kBQ >> p.split_log2;
+    const bool live = w.p0 + t < p.P;
+    const long long row0 = (C::kWeight ? static_cast<long long>(w.e) * p.Q + w.q0 : w.row0) + rank * per;
+    const int n = min(per, w.cnt - rank * per);
+    T* ptr = static_cast<T*>(p.out) + row0 * p.P + w.p0 + t;
+    const uint32_t* part = red + t * V;
+#pragma unroll 2
+    for (int cl = 0; cl < n; cl += V) {
+        float x[V];
+        if constexpr (C::kKind == kKindI8) {
+            int sum[V] = {};
+#pragma unroll 2
+            for (int s = 0; s < S; ++s)
+#pragma unroll
+                for (int i = 0; i < V; ++i) sum[i] += static_cast<int>(part[(s * per + cl) * 128 + i]);
+#pragma unroll
+            for (int i = 0; i < V; ++i) x[i] = fmaf(__int2float_rn(sum[i]) * scale[cl + i], sp, bias);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) x[i] = 0.f;
+#pragma unroll 2
+            for (int s = 0; s < S; ++s)
+#pragma unroll
+                for (int i = 0; i < V; ++i) x[i] += __uint_as_float(part[(s * per + cl) * 128 + i]);
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            if (cl + i < n && live) *ptr = T(x[i]);
+            ptr += p.P;
+        }
+    }
+}
+
+template <class C, class T>
+__device__ __forceinline__ void finish(const RowsParams& p, const RowsItem& w, const uint32_t* red, const float* scale,
+                                       int rank, int t, float sp, float bias)
+{
+    if ((C::kBQ >> p.split_log2) >= 4)
+        finish_parts<C, 4, T>(p, w, red, scale, rank, t, sp, bias);
+    else
+        finish_parts<C, 2, T>(p, w, red, scale, rank, t, sp, bias);
+}
+
 template <class C>
 __global__ void __launch_bounds__(C::kThreads, 1)
     rows_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ CUtensorMap tmQ,
@@ -312,38 +418,43 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                ~static_cast<uintptr_t>(1023));
-    const int S = C::kSub == 1 ? p.split : 1;
-    uint32_t* red = reinterpret_cast<uint32_t*>(smem + C::kRingBytes);
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kRingBytes + (S > 1 ? C::kRedBytes : 0));
-    uint64_t* empty = full + C::kStages;
-    uint64_t* conv = empty + C::kStages;     // kConv: stage widened (one arrival per converter warp)
-    uint64_t* tfull = conv + C::kStages;     // accumulator block h complete
+    const int S = C::kSub == 1 ? 1 << p.split_log2 : 1;
+    const int stages = p.stages;
+    uint32_t* red = reinterpret_cast<uint32_t*>(smem + stages * C::kStageBytes);
+    float* red_scale = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(red) + (S > 1 ? C::kRedBytes : 0));
+    uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(red_scale) + (S > 1 ? C::kScaleBytes : 0));
+    uint64_t* empty = full + C::kMaxStages;
+    uint64_t* conv = empty + C::kMaxStages;  // kConv: stage widened (one arrival per converter warp)
+    uint64_t* tfull = conv + C::kMaxStages;  // accumulator block h complete
     uint64_t* tempty = tfull + 2;            // accumulator block h read
     uint64_t* drain = tempty + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
     volatile uint32_t* abort_flag = tmem_slot + 1;
     int* bound = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(full) + C::kBarBytes);
-    int* cum = bound + p.groups + 3;
+    int* cum = bound + p.groups + 3;  // (used, and room for it, with offsets only)
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     const int rank = S > 1 ? static_cast<int>(cluster_ctarank()) : 0;
 
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < C::kStages; ++s) {
-            mbar_init(smem_u32(&full[s]), 1);
-            mbar_init(smem_u32(&empty[s]), 1);
-            mbar_init(smem_u32(&conv[s]), C::kConvWarps ? C::kConvWarps : 1);
+    if (warp == 0) {
+        // one barrier a lane: full, empty, conv of a stage; then the others
+        if (lane < stages) {
+            mbar_init(smem_u32(&full[lane]), 1);
+            mbar_init(smem_u32(&empty[lane]), 1);
+            if (C::kConv) mbar_init(smem_u32(&conv[lane]), C::kConvWarps);
+        } else if (lane >= 16 && lane < 18) {
+            mbar_init(smem_u32(&tfull[lane - 16]), 1);
+            mbar_init(smem_u32(&tempty[lane - 16]), 4);
+        } else if (lane == 18) {
+            mbar_init(smem_u32(drain), 1);
+            *abort_flag = 0u;
+        } else if (lane == 19) {
+            tma_prefetch_desc(&tmP);
+        } else if (lane == 20) {
+            tma_prefetch_desc(&tmQ);
         }
-        for (int h = 0; h < 2; ++h) {
-            mbar_init(smem_u32(&tfull[h]), 1);
-            mbar_init(smem_u32(&tempty[h]), 4);
-        }
-        mbar_init(smem_u32(drain), 1);
-        *abort_flag = 0u;
         fence_mbar_init();
-        tma_prefetch_desc(&tmP);
-        tma_prefetch_desc(&tmQ);
     }
     if (warp == 1) {
         tmem_alloc(smem_u32(tmem_slot), C::kTmemCols);
@@ -362,13 +473,23 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     const uint32_t tmem_base = *tmem_slot;
     const uint32_t ring = smem_u32(smem);
 
-    const int total = rows_total<C>(p, cum);
-    const int first = static_cast<int>(blockIdx.x) / S;
-    const int stride = static_cast<int>(gridDim.x) / S;
+    // kSub = 1: one tile a CTA, by its place in the grid (x: q-tile and rank, y:
+    // p-tile, z: group of the weight form); kSub = 2: items from here on.
+    const int qtiles = rows_qtiles<C>(p, cum);
+    const int tq1 = static_cast<int>(blockIdx.x) >> p.split_log2;
+    const int first = C::kSub == 1 ? 0 : static_cast<int>(blockIdx.x);
+    const int stride = C::kSub == 1 ? 1 : static_cast<int>(gridDim.x);
+    const int total = C::kSub == 1 ? ((C::kWeight ? p.qtiles : qtiles) > tq1 ? 1 : 0) : qtiles * p.ptiles;
+    const auto tile_of = [&](int item) {
+        if constexpr (C::kSub == 1)
+            return rows_tile<C>(p, static_cast<int>(blockIdx.y), tq1, static_cast<int>(blockIdx.z), bound, cum);
+        else
+            return rows_item<C>(p, item, qtiles, bound, cum);
+    };
     // this CTA's share [kb0, kb1) of a tile's k-blocks
     const auto share = [&](const RowsItem& w, int& kb0, int& kb1) {
-        kb0 = static_cast<int>(static_cast<long long>(w.nkb) * rank / S);
-        kb1 = static_cast<int>(static_cast<long long>(w.nkb) * (rank + 1) / S);
+        kb0 = C::kSub == 1 ? (w.nkb * rank) >> p.split_log2 : 0;
+        kb1 = C::kSub == 1 ? (w.nkb * (rank + 1)) >> p.split_log2 : w.nkb;
     };
     const auto blocks_of = [&](const RowsItem& w) { return C::kSub == 2 && p.P - w.p0 > 128 ? 2 : 1; };
     // length of the sum inside k-block kb
@@ -378,8 +499,9 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     };
     uint32_t issued = 0, issued_parity = 0;  // producer: loads in flight, for the abort path
 
-    if (threadIdx.x == 0) {
+    if (warp == 0) {
         // ---------------------------------------------------- producer ----
+        if (elect_one()) {
         int stage = 0;
         uint32_t phase = 0;
         bool aborted = false;
@@ -410,7 +532,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
         };
         bool waited = !p.early;
         for (int item = first; item < total && !aborted; item += stride) {
-            const RowsItem w = rows_item<C>(p, item, total, bound, cum);
+            const RowsItem w = tile_of(item);
             int kb0, kb1;
             share(w, kb0, kb1);
             const int blocks = blocks_of(w);
@@ -420,7 +542,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
             int kb = kb0;
             if (!waited) {
                 // the first ring-full: features now, rows once the kernel before has finished
-                const int ahead = kb1 - kb0 < C::kStages ? kb1 - kb0 : C::kStages;
+                const int ahead = kb1 - kb0 < stages ? kb1 - kb0 : stages;
                 for (int i = 0; i < ahead; ++i) {
                     mbar_arrive_expect_tx(smem_u32(&full[i]), tx);
                     load_p(w, kb0 + i, i, blocks);
@@ -433,7 +555,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
                 }
                 kb += ahead;
                 stage = ahead;
-                if (stage == C::kStages) stage = 0, phase = 1u;
+                if (stage == stages) stage = 0, phase = 1u;
             }
             for (; kb < kb1; ++kb) {
                 if (!wait_bounded(smem_u32(&empty[stage]), phase ^ 1u, abort_flag, p.timeout_ns,
@@ -446,17 +568,18 @@ __global__ void __launch_bounds__(C::kThreads, 1)
                 load_q(w, kb, stage, boxes);
                 issued |= 1u << stage;
                 issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
-                if (++stage == C::kStages) stage = 0, phase ^= 1u;
+                if (++stage == stages) stage = 0, phase ^= 1u;
             }
         }
         if (!waited) grid_dependency_wait();
         // Tail: every stage filled has been released, so no MMA commit arrives
         // on this CTA's barriers after it exits.
-        for (int i = 0; i < C::kStages && !aborted; ++i) {
+        for (int i = 0; i < stages && !aborted; ++i) {
             if (!wait_bounded(smem_u32(&empty[stage]), phase ^ 1u, abort_flag, p.timeout_ns,
                               (blockIdx.x << 8) | 0x50u | stage))
                 break;
-            if (++stage == C::kStages) stage = 0, phase ^= 1u;
+            if (++stage == stages) stage = 0, phase ^= 1u;
+        }
         }
     } else if (warp == 1) {
         // -------------------------------------------------- MMA issuer ----
@@ -464,8 +587,11 @@ __global__ void __launch_bounds__(C::kThreads, 1)
         uint32_t phase = 0;
         uint32_t acc_phase = 0;
         bool aborted = false;
+        const uint64_t pdesc = C::kPMn ? smem_desc_sw128(ring, 8192, 1024) : smem_desc_sw128(ring, 16, 1024);
+        const uint64_t qdesc = C::kQMn ? smem_desc_sw128(ring + C::kPBytes, 8192, 1024)
+                                       : smem_desc_sw128(ring + C::kPBytes, 16, 1024);
         for (int item = first; item < total && !aborted; item += stride) {
-            const RowsItem w = rows_item<C>(p, item, total, bound, cum);
+            const RowsItem w = tile_of(item);
             int kb0, kb1;
             share(w, kb0, kb1);
             if (kb0 == kb1) continue;  // nothing to sum: the epilogue writes zeros
@@ -473,65 +599,137 @@ __global__ void __launch_bounds__(C::kThreads, 1)
             // columns of the MMA: the tile's rows rounded up to what the instruction takes
             const int n = w.cnt <= 16 ? 16 : (w.cnt + 31) & ~31;
             const uint32_t idesc = p.idesc | (static_cast<uint32_t>(n >> 3) << 17);
-            for (int h = 0; h < C::kSub; ++h)
-                if (!wait_bounded_warp(smem_u32(&tempty[h]), acc_phase ^ 1u, abort_flag, p.timeout_ns,
-                                       (blockIdx.x << 8) | 0x20u | h)) {
-                    aborted = true;
-                    break;
-                }
-            if (aborted) break;
-            tc_fence_after();
-            for (int kb = kb0; kb < kb1; ++kb) {
-                if (!wait_bounded_warp(smem_u32(&full[stage]), phase, abort_flag, p.timeout_ns,
-                                       (blockIdx.x << 8) | 0x30u | stage)) {
-                    aborted = true;
-                    break;
-                }
-                if (C::kConv && !wait_bounded_warp(smem_u32(&conv[stage]), phase, abort_flag, p.timeout_ns,
-                                                   (blockIdx.x << 8) | 0x38u | stage)) {
-                    aborted = true;
-                    break;
-                }
+            // stage st, k-block kb: operands in shared memory
+            const auto ready = [&](int st, uint32_t ph) {
+                return wait_bounded_warp(smem_u32(&full[st]), ph, abort_flag, p.timeout_ns,
+                                         (blockIdx.x << 8) | 0x30u | st) &&
+                       (!C::kConv || wait_bounded_warp(smem_u32(&conv[st]), ph, abort_flag, p.timeout_ns,
+                                                       (blockIdx.x << 8) | 0xB0u | st));
+            };
+            // The sum ends inside an MMA step of the last k-block: the step's
+            // remaining rows belong to the next group and are overwritten with
+            // zeros, in both operands (0 x NaN would not be 0).
+            const auto clear_rest = [&](int st, int kb) {
                 const int valid = valid_of(w, kb);
-                const int ksteps = (valid + C::kUmmaK - 1) / C::kUmmaK;
-                uint8_t* st = smem + stage * C::kStageBytes;
-                if (C::kWeight && (valid & 15)) {
-                    // The sum ends inside an MMA step: the step's remaining
-                    // rows belong to the next group and are overwritten with
-                    // zeros, in both operands (0 x NaN would not be 0).
-                    const int extra = 16 - (valid & 15);
-                    const int atoms = (C::kConv ? 0 : 2 * blocks) + (n + 63) / 64;
-                    for (int i = lane; i < atoms * extra * 8; i += 32) {
-                        const int a = i / (extra * 8), r = valid + (i / 8) % extra;
-                        const int pa = C::kConv ? 0 : 2 * blocks;
-                        uint8_t* atom = a < pa ? st + a * 8192 : st + C::kPBytes + (a - pa) * 8192;
-                        *reinterpret_cast<uint4*>(atom + r * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                    fence_proxy_async_smem();
-                    __syncwarp();
+                if (!C::kWeight || (valid & 15) == 0) return;
+                uint8_t* base = smem + st * C::kStageBytes;
+                const int extra = 16 - (valid & 15);
+                const int pa = C::kConv ? 0 : 2 * blocks;
+                for (int i = lane; i < (pa + (n + 63) / 64) * extra * 8; i += 32) {
+                    const int a = i / (extra * 8), r = valid + (i / 8) % extra;
+                    uint8_t* atom = a < pa ? base + a * 8192 : base + C::kPBytes + (a - pa) * 8192;
+                    *reinterpret_cast<uint4*>(atom + r * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
                 }
+                fence_proxy_async_smem();
+                __syncwarp();
+            };
+            // the MMAs of k-block kb in stage st into the accumulator blocks of
+            // `mask`; a descriptor's low word is an address in 16-byte units
+            const auto issue = [&](int st, int kb, int mask) {
                 tc_fence_after();
-                if (lane == 0) {
-                    const uint32_t pa = smem_u32(st), qa = pa + C::kPBytes;
-                    for (int k = 0; k < ksteps; ++k) {
-                        const uint64_t qd = C::kQMn ? smem_desc_sw128(qa + k * C::kUmmaK * 128, 8192, 1024)
-                                                    : smem_desc_sw128(qa + k * 32, 16, 1024);
-                        for (int h = 0; h < blocks; ++h) {
-                            const uint32_t ph = pa + h * C::kSubBytes;
-                            const uint64_t pd = C::kPMn ? smem_desc_sw128(ph + k * C::kUmmaK * 128, 8192, 1024)
-                                                        : smem_desc_sw128(ph + k * 32, 16, 1024);
-                            umma<C::kKind>(tmem_base + h * C::kBQ, pd, qd, idesc, kb > kb0 || k > 0 ? 1u : 0u);
-                        }
+                if (elect_one()) {
+                    const int ksteps = (valid_of(w, kb) + C::kUmmaK - 1) / C::kUmmaK;
+                    const uint64_t at = static_cast<uint64_t>(st) * (C::kStageBytes / 16);
+#pragma unroll
+                    for (int k = 0; k < C::kBK / C::kUmmaK; ++k) {
+                        if (k >= ksteps) break;
+                        const uint64_t qd = qdesc + at + k * (C::kQMn ? C::kUmmaK * 8 : 2);
+                        const uint64_t pd = pdesc + at + k * (C::kPMn ? C::kUmmaK * 8 : 2);
+                        const uint32_t sum = kb > kb0 || k > 0 ? 1u : 0u;
+                        if (mask & 1) umma<C::kKind>(tmem_base, pd, qd, idesc, sum);
+                        if (C::kSub == 2 && (mask & 2))
+                            umma<C::kKind>(tmem_base + C::kBQ, pd + C::kSubBytes / 16, qd, idesc, sum);
                     }
-                    umma_commit(smem_u32(&empty[stage]));
                 }
                 __syncwarp();
-                if (++stage == C::kStages) stage = 0, phase ^= 1u;
+            };
+            const auto release = [&]() {
+                if (elect_one()) umma_commit(smem_u32(&empty[stage]));
+                __syncwarp();
+                if (++stage == stages) stage = 0, phase ^= 1u;
+            };
+            const auto complete = [&](int h) {
+                if (elect_one()) umma_commit(smem_u32(&tfull[h]));
+                __syncwarp();
+            };
+            if (!wait_bounded_warp(smem_u32(&tempty[0]), acc_phase ^ 1u, abort_flag, p.timeout_ns,
+                                   (blockIdx.x << 8) | 0x20u))
+                break;
+            const int mask = blocks == 2 ? 3 : 1;
+            int kb = kb0;
+            if constexpr (C::kSub == 2) {
+                // Both accumulators belong to one tile, so the epilogue has to
+                // overlap the MMAs of the other block: while block 1 is still
+                // being read, k-blocks go into block 0 only (their stages stay
+                // held) and into block 1 once it is free; and the last k-blocks
+                // go into block 0 first, so its epilogue starts early.
+                const int pre = kb1 - kb0 < stages ? kb1 - kb0 : stages;
+                int held = 0, st = stage;
+                uint32_t ph = phase;
+                const auto next = [&]() {
+                    if (++st == stages) st = 0, ph ^= 1u;
+                };
+                bool free1 = __all_sync(0xffffffffu, mbar_try_wait(smem_u32(&tempty[1]), acc_phase ^ 1u));
+                while (!free1 && held < pre) {
+                    if (!ready(st, ph)) {
+                        aborted = true;
+                        break;
+                    }
+                    if (kb0 + held == kb1 - 1) clear_rest(st, kb0 + held);
+                    issue(st, kb0 + held, 1);
+                    ++held;
+                    next();
+                    free1 = __all_sync(0xffffffffu, mbar_try_wait(smem_u32(&tempty[1]), acc_phase ^ 1u));
+                }
+                if (aborted) break;
+                if (!free1 && !wait_bounded_warp(smem_u32(&tempty[1]), acc_phase ^ 1u, abort_flag, p.timeout_ns,
+                                                 (blockIdx.x << 8) | 0x21u))
+                    break;
+                for (; kb < kb0 + held; ++kb) {
+                    issue(stage, kb, mask & 2);
+                    release();
+                }
+                const int last = kb1 - kb < stages ? kb1 - kb : stages;
+                for (; kb < kb1 - last; ++kb) {
+                    if (!ready(stage, phase)) {
+                        aborted = true;
+                        break;
+                    }
+                    issue(stage, kb, mask);
+                    release();
+                }
+                if (aborted) break;
+                st = stage;
+                ph = phase;
+                for (int i = 0; i < last; ++i) {
+                    if (!ready(st, ph)) {
+                        aborted = true;
+                        break;
+                    }
+                    if (kb + i == kb1 - 1) clear_rest(st, kb + i);
+                    issue(st, kb + i, 1);
+                    next();
+                }
+                if (aborted) break;
+                complete(0);
+                for (; kb < kb1; ++kb) {
+                    issue(stage, kb, mask & 2);
+                    release();
+                }
+                complete(1);
+            } else {
+                for (; kb < kb1; ++kb) {
+                    if (!ready(stage, phase)) {
+                        aborted = true;
+                        break;
+                    }
+                    if (kb == kb1 - 1) clear_rest(stage, kb);
+                    issue(stage, kb, 1);
+                    release();
+                }
+                if (aborted) break;
+                complete(0);
             }
-            if (aborted) break;
-            if (lane == 0)
-                for (int h = 0; h < C::kSub; ++h) umma_commit(smem_u32(&tfull[h]));
-            __syncwarp();
             acc_phase ^= 1u;
         }
     } else if (warp >= 2 && warp < 6) {
@@ -541,7 +739,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
         bool lost = false;
         if (p.early) grid_dependency_wait();  // the rows' scales, and the output's last readers
         for (int item = first; item < total && !lost; item += stride) {
-            const RowsItem w = rows_item<C>(p, item, total, bound, cum);
+            const RowsItem w = tile_of(item);
             int kb0, kb1;
             share(w, kb0, kb1);
             const bool empty_sum = kb0 == kb1;
@@ -577,18 +775,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
                     }
                     const int n = w.cnt - c < 32 ? w.cnt - c : 32;
                     if (C::kSub == 1 && S > 1) {
-                        // this CTA's part of column c + j to the CTA that
-                        // finishes that column: [source rank][column][feature]
-                        const int per = C::kBQ / S;
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            if (j < n) {
-                                const int d = (c + j) / per, cl = (c + j) - d * per;
-                                const uint32_t at =
-                                    smem_u32(red + (rank * per + cl) * 128 + quarter * 32 + lane);
-                                st_cluster_u32(mapa_shared(at, d), v[j]);
-                            }
-                        }
+                        push_part<C>(v, red, rank, p.split_log2, c, n, quarter * 32 + lane);
                         continue;
                     }
                     float sq = 0.f;
@@ -618,7 +805,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
         uint32_t phase = 0;
         bool ok = true;
         for (int item = first; item < total && ok; item += stride) {
-            const RowsItem w = rows_item<C>(p, item, total, bound, cum);
+            const RowsItem w = tile_of(item);
             int kb0, kb1;
             share(w, kb0, kb1);
             for (int kb = kb0; kb < kb1; ++kb) {
@@ -644,7 +831,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&conv[stage]));
-                if (++stage == C::kStages) stage = 0, phase ^= 1u;
+                if (++stage == stages) stage = 0, phase ^= 1u;
             }
         }
     }
@@ -654,56 +841,47 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     if (*abort_flag) {
         // Some role gave up.  Before shared and tensor memory are released,
         // let this CTA's own copies land and its MMAs retire.
-        if (threadIdx.x == 0)
-            for (int s = 0; s < C::kStages; ++s)
-                if (issued & (1u << s)) drain_wait(smem_u32(&full[s]), (issued_parity >> s) & 1u);
-        if (threadIdx.x == 32) {
-            umma_commit(smem_u32(drain));
-            drain_wait(smem_u32(drain), 0);
+        // (`issued` is zero in every thread but the producer; elect_one picks
+        // the same lane of the converged warp that issued the MMAs)
+        for (int s = 0; s < stages; ++s)
+            if (issued & (1u << s)) drain_wait(smem_u32(&full[s]), (issued_parity >> s) & 1u);
+        __syncwarp();
+        if (warp == 1) {
+            if (elect_one()) {
+                umma_commit(smem_u32(drain));
+                drain_wait(smem_u32(drain), 0);
+            }
         }
         __syncwarp();
         __syncthreads();
     }
     if (C::kSub == 1 && S > 1) {
-        cluster_sync_all();  // every part has arrived
-        if (first < total && !*abort_flag) {
-            // this CTA's columns of the tile: the parts in rank order
-            const RowsItem w = rows_item<C>(p, first, total, bound, cum);
-            const int per = C::kBQ / S;
-            const int f = w.p0 + (static_cast<int>(threadIdx.x) & 127);
-            if (threadIdx.x < 128 && f < p.P) {
-                float sp = 0.f, bias = 0.f;
-                if (C::kKind == kKindI8 && !w.zero) {
-                    const long long at = static_cast<long long>(w.e) * p.P + f;
+        const bool work = total > 0 && !*abort_flag;
+        RowsItem w;
+        float sp = 0.f, bias = 0.f;
+        const int per = C::kBQ >> p.split_log2;
+        const int t = static_cast<int>(threadIdx.x);
+        if (work) {
+            w = tile_of(0);
+            if (C::kKind == kKindI8) {
+                if (t < 128 && w.p0 + t < p.P && !w.zero) {
+                    const long long at = static_cast<long long>(w.e) * p.P + w.p0 + t;
                     sp = p.scale_p[at];
                     if (p.bias_p) bias = p.bias_p[at];
                 }
                 if (p.early) grid_dependency_wait();
-                const long long row0 = C::kWeight ? static_cast<long long>(w.e) * p.Q + w.q0 : w.row0;
-                for (int cl = 0; cl < per; ++cl) {
-                    const int c = rank * per + cl;
-                    if (c >= w.cnt) break;
-                    float x;
-                    if constexpr (C::kKind == kKindI8) {
-                        int sum = 0;
-                        for (int s = 0; s < S; ++s)
-                            sum += static_cast<int>(red[(s * per + cl) * 128 + threadIdx.x]);
-                        const float sq = w.zero ? 0.f : p.scale_q[w.row0 + c];
-                        x = fmaf(__int2float_rn(sum) * sq, sp, bias);
-                    } else {
-                        x = 0.f;
-                        for (int s = 0; s < S; ++s)
-                            x += __uint_as_float(red[(s * per + cl) * 128 + threadIdx.x]);
-                    }
-                    const long long at = (row0 + c) * p.P + f;
-                    if (p.out_type == kOutF32)
-                        static_cast<float*>(p.out)[at] = x;
-                    else if (p.out_type == kOutF16)
-                        static_cast<__half*>(p.out)[at] = __float2half_rn(x);
-                    else
-                        static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(x);
-                }
+                if (t < per)
+                    red_scale[t] = rank * per + t < w.cnt && !w.zero ? p.scale_q[w.row0 + rank * per + t] : 0.f;
             }
+        }
+        cluster_sync_all();  // every part has arrived
+        if (work && t < 128) {
+            if (p.out_type == kOutF32)
+                finish<C, float>(p, w, red, red_scale, rank, t, sp, bias);
+            else if (p.out_type == kOutF16)
+                finish<C, __half>(p, w, red, red_scale, rank, t, sp, bias);
+            else
+                finish<C, __nv_bfloat16>(p, w, red, red_scale, rank, t, sp, bias);
         }
     }
     tc_fence_after();
