@@ -28,9 +28,9 @@
 //   kSub = 2: 256 x 256, persistent CTAs, two M = 128 accumulators that fill
 //     the tensor memory.  For many rows, where the tensor cores bound it.
 //
-// Warps: 0 TMA producer (one thread), 1 MMA issuer, 2..5 epilogue (one per
+// Warps: 0 TMA producer (one thread), 1 MMA issuer, 2..9 epilogue (two per
 // tensor-memory lane quarter), and with kConv eight converter warps (see
-// conv_tile).  Every wait on an mbarrier is bounded (tcg_wait.cuh).
+// conv_write).  Every wait on an mbarrier is bounded (tcg_wait.cuh).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -85,7 +85,10 @@ struct RowsTraits {
     static constexpr int kQBoxBytes = kQBox * 128;
     static constexpr int kRawBytes = 128 * kBK;         // kConv: int8 codes of one 128-feature block
     static constexpr int kConvWarps = kConv ? 8 : 0;
-    static constexpr int kThreads = 192 + 32 * kConvWarps;
+    static constexpr int kEpiWarps = 8;                 // two per quarter of the tensor memory's lanes
+    static constexpr int kFirstConv = 2 + kEpiWarps;
+    static constexpr int kThreads = 32 * (kFirstConv + kConvWarps);
+    static constexpr int kPerSm = kSub == 1 && !kConv ? 2 : 1;  // CTAs per SM that registers are kept for
     static constexpr int kTmemCols = kSub * kBQ < 32 ? 32 : kSub * kBQ;
     static constexpr int kRedBytes = kBQ * 512;         // split: 128 x kBQ partial sums
     static constexpr int kMaxStages = 12;
@@ -361,20 +364,20 @@ __device__ __forceinline__ void push_part(const uint32_t (&v)[32], uint32_t* red
 }
 
 // This CTA's columns of the tile: the parts added in rank order, scaled, and
-// stored; one thread per feature, V columns at a time.
+// stored; two threads per feature f, V columns at a time in turn (g).
 template <class C, int V, class T>
 __device__ __forceinline__ void finish_parts(const RowsParams& p, const RowsItem& w, const uint32_t* red,
-                                             const float* scale, int rank, int t, float sp, float bias)
+                                             const float* scale, int rank, int f, int g, float sp, float bias)
 {
     const int S = 1 << p.split_log2;
     const int per = C::kBQ >> p.split_log2;
-    const bool live = w.p0 + t < p.P;
+    const bool live = w.p0 + f < p.P;
     const long long row0 = (C::kWeight ? static_cast<long long>(w.e) * p.Q + w.q0 : w.row0) + rank * per;
     const int n = min(per, w.cnt - rank * per);
-    T* ptr = static_cast<T*>(p.out) + row0 * p.P + w.p0 + t;
-    const uint32_t* part = red + t * V;
+    T* ptr = static_cast<T*>(p.out) + (row0 + g * V) * p.P + w.p0 + f;
+    const uint32_t* part = red + f * V;
 #pragma unroll 2
-    for (int cl = 0; cl < n; cl += V) {
+    for (int cl = g * V; cl < n; cl += 2 * V) {
         float x[V];
         if constexpr (C::kKind == kKindI8) {
             int sum[V] = {};
@@ -397,6 +400,7 @@ __device__ __forceinline__ void finish_parts(const RowsParams& p, const RowsItem
             if (cl + i < n && live) *ptr = T(x[i]);
             ptr += p.P;
         }
+        ptr += static_cast<long long>(V) * p.P;
     }
 }
 
@@ -405,13 +409,13 @@ __device__ __forceinline__ void finish(const RowsParams& p, const RowsItem& w, c
                                        int rank, int t, float sp, float bias)
 {
     if ((C::kBQ >> p.split_log2) >= 4)
-        finish_parts<C, 4, T>(p, w, red, scale, rank, t, sp, bias);
+        finish_parts<C, 4, T>(p, w, red, scale, rank, t & 127, t >> 7, sp, bias);
     else
-        finish_parts<C, 2, T>(p, w, red, scale, rank, t, sp, bias);
+        finish_parts<C, 2, T>(p, w, red, scale, rank, t & 127, t >> 7, sp, bias);
 }
 
 template <class C>
-__global__ void __launch_bounds__(C::kThreads, 1)
+__global__ void __launch_bounds__(C::kThreads, C::kPerSm)
     rows_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ CUtensorMap tmQ,
                 const __grid_constant__ RowsParams p)
 {
@@ -445,7 +449,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
             if (C::kConv) mbar_init(smem_u32(&conv[lane]), C::kConvWarps);
         } else if (lane >= 16 && lane < 18) {
             mbar_init(smem_u32(&tfull[lane - 16]), 1);
-            mbar_init(smem_u32(&tempty[lane - 16]), 4);
+            mbar_init(smem_u32(&tempty[lane - 16]), C::kEpiWarps);
         } else if (lane == 18) {
             mbar_init(smem_u32(drain), 1);
             *abort_flag = 0u;
@@ -732,9 +736,10 @@ __global__ void __launch_bounds__(C::kThreads, 1)
             }
             acc_phase ^= 1u;
         }
-    } else if (warp >= 2 && warp < 6) {
+    } else if (warp >= 2 && warp < C::kFirstConv) {
         // ---------------------------------------------------- epilogue ----
         const int quarter = warp & 3;
+        const int c0 = ((warp - 2) >> 2) * 32;  // the two warps of a quarter take turns of 32 columns
         uint32_t acc_phase = 0;
         bool lost = false;
         if (p.early) grid_dependency_wait();  // the rows' scales, and the output's last readers
@@ -764,7 +769,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
                 const uint32_t t_addr =
                     tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(h * C::kBQ);
 #pragma unroll 1
-                for (int c = 0; c < w.cnt; c += 32) {
+                for (int c = c0; c < w.cnt; c += 64) {
                     uint32_t v[32];
                     if (empty_sum) {
 #pragma unroll
@@ -796,11 +801,11 @@ __global__ void __launch_bounds__(C::kThreads, 1)
             }
             if (!empty_sum) acc_phase ^= 1u;
         }
-    } else if (C::kConv && warp >= 6) {
+    } else if (C::kConv && warp >= C::kFirstConv) {
         // -------------------------------------------------- converters ----
         // Every wait's outcome goes through a barrier-AND of the converter
         // warps, so they give up together.
-        const int ct = static_cast<int>(threadIdx.x) - 192;
+        const int ct = static_cast<int>(threadIdx.x) - 32 * C::kFirstConv;
         int stage = 0;
         uint32_t phase = 0;
         bool ok = true;
@@ -864,8 +869,8 @@ __global__ void __launch_bounds__(C::kThreads, 1)
         if (work) {
             w = tile_of(0);
             if (C::kKind == kKindI8) {
-                if (t < 128 && w.p0 + t < p.P && !w.zero) {
-                    const long long at = static_cast<long long>(w.e) * p.P + w.p0 + t;
+                if (t < 256 && w.p0 + (t & 127) < p.P && !w.zero) {
+                    const long long at = static_cast<long long>(w.e) * p.P + w.p0 + (t & 127);
                     sp = p.scale_p[at];
                     if (p.bias_p) bias = p.bias_p[at];
                 }
@@ -875,7 +880,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
             }
         }
         cluster_sync_all();  // every part has arrived
-        if (work && t < 128) {
+        if (work && t < 256) {
             if (p.out_type == kOutF32)
                 finish<C, float>(p, w, red, red_scale, rank, t, sp, bias);
             else if (p.out_type == kOutF16)
