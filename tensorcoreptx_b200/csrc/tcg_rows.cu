@@ -130,6 +130,8 @@ tcg_status launch(const RowsCall& c, int split, int dev, int sms, cudaStream_t s
     p.ptiles = ceil_div(c.P, C::kTileP);
     p.qtiles = ceil_div(C::kWeight ? c.Q : p.rows_per_group, C::kBQ);
     p.zero_rest = c.zero_rest;
+    const int out_bytes = c.out_type == kOutF32 ? 4 : 2;
+    p.aligned_out = (static_cast<long long>(c.P) * out_bytes) % 16 == 0 && (reinterpret_cast<uintptr_t>(c.out) & 15u) == 0;
     p.out_type = c.out_type;
     p.bf16 = c.bf16;
     while ((1 << p.split_log2) < split) ++p.split_log2;

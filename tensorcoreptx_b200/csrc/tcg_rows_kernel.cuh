@@ -59,6 +59,7 @@ struct RowsParams {
     int band_log2;            // kSub = 2: tiles along q per rasterisation band
     uint32_t per_band_inv, ptiles_inv, per_group_inv;  // div_by: band * ptiles, ptiles, tiles per group
     int zero_rest;            // rows form: write zeros into rows outside every group
+    int aligned_out;          // output rows are whole 16-byte vectors, 16-byte aligned
     int out_type;
     int bf16;                 // 16-bit operands are bf16 (kConv: type of the widened codes)
     int split_log2;           // kSub = 1: 1, 2, 4 or 8 CTAs per tile
@@ -88,12 +89,17 @@ struct RowsTraits {
     static constexpr int kEpiWarps = 8;                 // two per quarter of the tensor memory's lanes
     static constexpr int kFirstConv = 2 + kEpiWarps;
     static constexpr int kThreads = 32 * (kFirstConv + kConvWarps);
+    // 16-bit results of a whole tile fit the epilogue's registers
+    static constexpr bool kHold = kSub == 2 && !kConv;
     static constexpr int kPerSm = kSub == 1 && !kConv ? 2 : 1;  // CTAs per SM that registers are kept for
     static constexpr int kTmemCols = kSub * kBQ < 32 ? 32 : kSub * kBQ;
     static constexpr int kRedBytes = kBQ * 512;         // split: 128 x kBQ partial sums
     static constexpr int kMaxStages = 12;
     static constexpr int kBarBytes = 384;
-    static constexpr int kScaleBytes = 512;             // split: scales of the rows a CTA finishes
+    static constexpr int kScaleBytes = 1024;            // scales of the rows being written out
+    // two blocks of 32 x 128 results on their way out; one tile a CTA: in the ring, which is idle by then
+    static constexpr int kOutBytes = 8192;
+    static constexpr int kOutArea = kSub == 2 ? 2 * kOutBytes : 0;
     static_assert(!kConv || (kPMn && kQMn && kKind == kKindF16), "converted operand: weight form only");
     static_assert(!kQMn || kKind == kKindF16, "weight form: 16-bit operands");
     static_assert(!kPMn || kKind == kKindF16, "MN-major features: 16-bit operands");
@@ -103,7 +109,8 @@ struct RowsTraits {
     // dynamic shared memory of a launch with a table of `groups` groups
     static constexpr int smem_bytes(int stages, int split, int groups)
     {
-        return 1024 + stages * kStageBytes + (split > 1 ? kRedBytes + kScaleBytes : 0) + kBarBytes + 8 * (groups + 3);
+        return 1024 + stages * kStageBytes + kOutArea + (split > 1 ? kRedBytes : 0) + kScaleBytes + kBarBytes +
+               8 * (groups + 3);
     }
 };
 
@@ -241,30 +248,123 @@ __device__ __forceinline__ RowsItem rows_item(const RowsParams& p, int item, int
     return rows_tile<C>(p, pt, tq, e, bound, cum);
 }
 
-// 32 accumulator words of one lane (one feature, columns c .. c + 31 of the
-// tile) to the output type and out: column j is row j of the output, where the
-// warp's 32 lanes write 32 consecutive elements.
-template <class C, class T>
-__device__ __forceinline__ void store_cols(const uint32_t (&v)[32], T* ptr, long long ld, int n, bool live, float sp,
-                                           float bias, float sq_lane)
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack16(float a, float b)
+{
+    if (kBf16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Results of 32 columns (rows of the output) x 128 features, held by the four
+// warps of one epilogue group as one feature a lane, out to memory with whole
+// 128-byte lines a warp: through 8 KB of shared memory, 16 x 128 words at a
+// time -- for 16-bit results a word is one feature of two rows.  (Straight from
+// the registers a warp's store is 64 bytes of one row, and the stores, not the
+// tensor cores, bound products with K < 8192: int8 8192 x 8192 x 1024 took
+// 101 us that way.)
+struct OutBlock {
+    void* out;
+    long long row;   // first row
+    int ld;          // elements
+    int f;           // first feature of the block
+    int n;           // rows of the block that exist
+    int features;    // features of the block that exist (<= 128)
+    bool aligned;    // rows are whole 16-byte vectors, 16-byte aligned
+};
+
+__device__ __forceinline__ void group_sync(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
+
+// two rows' values of one feature per word, each rounded once
+__device__ __forceinline__ void pack_block(const float (&x)[32], bool bf16, uint32_t (&w)[16])
+{
+    if (bf16) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) w[j] = pack16<true>(x[2 * j], x[2 * j + 1]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) w[j] = pack16<false>(x[2 * j], x[2 * j + 1]);
+    }
+}
+
+__device__ __forceinline__ void store_block16(const uint32_t (&w)[16], const OutBlock& o, uint32_t* stage, int quarter,
+                                              int lane, int barrier)
 {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-        float f;
-        if constexpr (C::kKind == kKindI8) {
-            // the int32 sum, rounded to fp32 once, times both scales, plus the bias
-            const float sq = __shfl_sync(0xffffffffu, sq_lane, j);
-            f = fmaf(__int2float_rn(static_cast<int>(v[j])) * sq, sp, bias);
-        } else {
-            f = __uint_as_float(v[j]);
+    for (int j = 0; j < 16; ++j) stage[j * 128 + quarter * 32 + lane] = w[j];
+    group_sync(barrier);
+    unsigned short* out = static_cast<unsigned short*>(o.out) + o.row * o.ld + o.f;
+    if (o.aligned) {
+        // 16 lanes a row pair, eight features a lane
+        const int e = (lane & 15) * 8;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int pair = quarter * 4 + i * 2 + (lane >> 4);
+            const uint4 a = *reinterpret_cast<const uint4*>(stage + pair * 128 + e);
+            const uint4 b = *reinterpret_cast<const uint4*>(stage + pair * 128 + e + 4);
+            unsigned short* row = out + static_cast<long long>(2 * pair) * o.ld + e;
+            if (e < o.features && 2 * pair < o.n)
+                *reinterpret_cast<uint4*>(row) =
+                    make_uint4(__byte_perm(a.x, a.y, 0x5410), __byte_perm(a.z, a.w, 0x5410),
+                               __byte_perm(b.x, b.y, 0x5410), __byte_perm(b.z, b.w, 0x5410));
+            if (e < o.features && 2 * pair + 1 < o.n)
+                *reinterpret_cast<uint4*>(row + o.ld) =
+                    make_uint4(__byte_perm(a.x, a.y, 0x7632), __byte_perm(a.z, a.w, 0x7632),
+                               __byte_perm(b.x, b.y, 0x7632), __byte_perm(b.z, b.w, 0x7632));
         }
-        if (j < n && live) {
-            if constexpr (sizeof(T) == 4)
-                *ptr = f;
-            else
-                *ptr = T(f);  // one rounding to nearest, at the end
+    } else {
+        // rows of odd length: aligned words of two features, and single ones at the ends
+#pragma unroll 1
+        for (int i = 0; i < 8; ++i) {
+            const int r = quarter * 8 + i;
+            if (r >= o.n) break;
+            unsigned short* row = out + static_cast<long long>(r) * o.ld;
+            const uint32_t* line = stage + (r >> 1) * 128;
+            const int shift = (r & 1) * 16;
+            const int odd = static_cast<int>(reinterpret_cast<uintptr_t>(row) >> 1) & 1;
+            if (odd && lane == 0) row[0] = static_cast<unsigned short>(line[0] >> shift);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int e = 2 * (lane + 32 * u) + odd;
+                if (e + 1 < o.features)
+                    *reinterpret_cast<uint32_t*>(row + e) =
+                        __byte_perm(line[e], line[e + 1], shift ? 0x7632 : 0x5410);
+                else if (e < o.features)
+                    row[e] = static_cast<unsigned short>(line[e] >> shift);
+            }
         }
-        ptr += ld;
+    }
+    group_sync(barrier);
+}
+
+__device__ __forceinline__ void store_block32(const float (&x)[32], const OutBlock& o, uint32_t* stage, int quarter,
+                                              int lane, int barrier)
+{
+    float* out = static_cast<float*>(o.out) + o.row * o.ld + o.f;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) stage[j * 128 + quarter * 32 + lane] = __float_as_uint(x[16 * half + j]);
+        group_sync(barrier);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = quarter * 4 + i;
+            float* row = out + static_cast<long long>(16 * half + r) * o.ld;
+            if (16 * half + r >= o.n) continue;
+            if (o.aligned) {
+                if (lane * 4 < o.features)
+                    *reinterpret_cast<uint4*>(row + lane * 4) =
+                        *reinterpret_cast<const uint4*>(stage + r * 128 + lane * 4);
+            } else {
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (lane + 32 * u < o.features) row[lane + 32 * u] = __uint_as_float(stage[r * 128 + lane + 32 * u]);
+            }
+        }
+        group_sync(barrier);
     }
 }
 
@@ -300,17 +400,6 @@ __device__ __forceinline__ float code_float(uint32_t w, int i)
 {
     // byte i of w (biased by 128) in the low mantissa bits of 2^23, minus 2^23 + 128: exact
     return __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7650 | i)) - 8388736.0f;
-}
-
-template <bool kBf16>
-__device__ __forceinline__ uint32_t pack16(float a, float b)
-{
-    if (kBf16) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    }
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 template <class C, bool kBf16>
@@ -424,9 +513,10 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                                                ~static_cast<uintptr_t>(1023));
     const int S = C::kSub == 1 ? 1 << p.split_log2 : 1;
     const int stages = p.stages;
-    uint32_t* red = reinterpret_cast<uint32_t*>(smem + stages * C::kStageBytes);
-    float* red_scale = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(red) + (S > 1 ? C::kRedBytes : 0));
-    uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(red_scale) + (S > 1 ? C::kScaleBytes : 0));
+    uint8_t* out_area = C::kSub == 2 ? smem + stages * C::kStageBytes : smem;
+    uint32_t* red = reinterpret_cast<uint32_t*>(smem + stages * C::kStageBytes + C::kOutArea);
+    float* scales = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(red) + (S > 1 ? C::kRedBytes : 0));
+    uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(scales) + C::kScaleBytes);
     uint64_t* empty = full + C::kMaxStages;
     uint64_t* conv = empty + C::kMaxStages;  // kConv: stage widened (one arrival per converter warp)
     uint64_t* tfull = conv + C::kMaxStages;  // accumulator block h complete
@@ -739,7 +829,9 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
     } else if (warp >= 2 && warp < C::kFirstConv) {
         // ---------------------------------------------------- epilogue ----
         const int quarter = warp & 3;
-        const int c0 = ((warp - 2) >> 2) * 32;  // the two warps of a quarter take turns of 32 columns
+        const int group = (warp - 2) >> 2;  // the two groups of four warps take 32 columns in turn
+        float* warp_scales = scales + (warp - 2) * 32;
+        uint32_t* stage_out = reinterpret_cast<uint32_t*>(out_area + group * C::kOutBytes);
         uint32_t acc_phase = 0;
         bool lost = false;
         if (p.early) grid_dependency_wait();  // the rows' scales, and the output's last readers
@@ -748,55 +840,127 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
             int kb0, kb1;
             share(w, kb0, kb1);
             const bool empty_sum = kb0 == kb1;
-            for (int h = 0; h < C::kSub; ++h) {
-                const int f = w.p0 + h * 128 + quarter * 32 + lane;  // this lane's feature
-                const bool live = f < p.P;
+            const long long row = C::kWeight ? static_cast<long long>(w.e) * p.Q + w.q0 : w.row0;
+            float sp = 0.f, bias = 0.f;  // of this lane's feature in the current block
+            // wait for block h of the accumulators
+            const auto begin = [&](int h) {
                 if (!empty_sum) {
-                    if (!wait_bounded_warp(smem_u32(&tfull[h]), acc_phase, abort_flag, p.timeout_ns,
-                                           (blockIdx.x << 8) | 0x40u | h)) {
+                    // (the four warps of a group agree on the outcome: none is
+                    // left waiting at a barrier that another has given up)
+                    const bool ok = wait_bounded_warp(smem_u32(&tfull[h]), acc_phase, abort_flag, p.timeout_ns,
+                                                      (blockIdx.x << 8) | 0x40u | h);
+                    if (!named_barrier_and(2 + group, 128, ok)) {
                         lost = true;
-                        break;
+                        return;
                     }
                     tc_fence_after();
                 }
-                float sp = 0.f, bias = 0.f;
-                if (C::kKind == kKindI8 && S == 1 && live && !w.zero) {
+                const int f = w.p0 + h * 128 + quarter * 32 + lane;
+                if (C::kKind == kKindI8 && S == 1 && f < p.P && !w.zero) {
                     const long long at = static_cast<long long>(w.e) * p.P + f;
                     sp = p.scale_p[at];
-                    if (p.bias_p) bias = p.bias_p[at];
+                    bias = p.bias_p ? p.bias_p[at] : 0.f;
                 }
-                const long long row = C::kWeight ? static_cast<long long>(w.e) * p.Q + w.q0 : w.row0;
-                const uint32_t t_addr =
-                    tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(h * C::kBQ);
-#pragma unroll 1
-                for (int c = c0; c < w.cnt; c += 64) {
-                    uint32_t v[32];
-                    if (empty_sum) {
+            };
+            // columns c .. c + 31 of block h
+            const auto load = [&](int h, int c, uint32_t (&v)[32]) {
+                if (empty_sum) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = 0u;
-                    } else {
-                        tmem_ld_32x32b_x32(t_addr + c, v);
-                        tmem_ld_wait();
-                    }
-                    const int n = w.cnt - c < 32 ? w.cnt - c : 32;
-                    if (C::kSub == 1 && S > 1) {
-                        push_part<C>(v, red, rank, p.split_log2, c, n, quarter * 32 + lane);
-                        continue;
-                    }
-                    float sq = 0.f;
-                    if (C::kKind == kKindI8 && !w.zero && lane < n) sq = p.scale_q[w.row0 + c + lane];
-                    const long long at = (row + c) * p.P + f;
-                    if (p.out_type == kOutF32)
-                        store_cols<C>(v, static_cast<float*>(p.out) + at, p.P, n, live, sp, bias, sq);
-                    else if (p.out_type == kOutF16)
-                        store_cols<C>(v, static_cast<__half*>(p.out) + at, p.P, n, live, sp, bias, sq);
-                    else
-                        store_cols<C>(v, static_cast<__nv_bfloat16*>(p.out) + at, p.P, n, live, sp, bias, sq);
+                    for (int j = 0; j < 32; ++j) v[j] = 0u;
+                } else {
+                    tmem_ld_32x32b_x32(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
+                                           static_cast<uint32_t>(h * C::kBQ + c),
+                                       v);
                 }
-                if (!empty_sum) {
-                    tc_fence_before();
+            };
+            const auto load_wait = [&]() {
+                if (!empty_sum) tmem_ld_wait();
+            };
+            const auto finish_load = [&](int c, uint32_t (&v)[32], float (&x)[32]) {
+                if (C::kKind == kKindI8) {  // the rows' scales, for every lane to read
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(&tempty[h]));
+                    warp_scales[lane] = !w.zero && c + lane < w.cnt ? p.scale_q[w.row0 + c + lane] : 0.f;
+                    __syncwarp();
+                }
+                load_wait();
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                    // int8: the int32 sum, rounded to fp32 once, times both scales, plus the bias
+                    if (C::kKind == kKindI8)
+                        x[j] = fmaf(__int2float_rn(static_cast<int>(v[j])) * warp_scales[j], sp, bias);
+                    else
+                        x[j] = __uint_as_float(v[j]);
+                }
+            };
+            const auto release = [&](int h) {
+                if (empty_sum) return;
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&tempty[h]));
+            };
+            const auto block_of = [&](int h, int c) {
+                return OutBlock{p.out, row + c, p.P, w.p0 + h * 128, min(32, w.cnt - c),
+                                min(128, p.P - w.p0 - h * 128), p.aligned_out != 0};
+            };
+            if (C::kHold && p.out_type != kOutF32) {
+                // Both blocks into registers (128 words a thread) before any
+                // store: the accumulators are free for the next tile after
+                // about 3000 cycles instead of the 11000 that the stores of
+                // all SMs at once take.
+                uint32_t held[2][4][16];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (lost) break;
+                    begin(h);
+                    if (lost) break;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int c = 32 * group + 64 * i;
+                        if (c < w.cnt) {
+                            uint32_t v[32];
+                            float x[32];
+                            load(h, c, v);
+                            finish_load(c, v, x);
+                            pack_block(x, p.out_type == kOutBF16, held[h][i]);
+                        }
+                    }
+                    release(h);
+                }
+                if (lost) break;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int c = 32 * group + 64 * i;
+                        const OutBlock o = block_of(h, c);
+                        if (c < w.cnt && o.features > 0) store_block16(held[h][i], o, stage_out, quarter, lane, 2 + group);
+                    }
+            } else {
+                for (int h = 0; h < C::kSub; ++h) {
+                    begin(h);
+                    if (lost) break;
+#pragma unroll 1
+                    for (int c = 32 * group; c < w.cnt; c += 64) {
+                        uint32_t v[32];
+                        load(h, c, v);
+                        if (C::kSub == 1 && S > 1) {
+                            load_wait();
+                            push_part<C>(v, red, rank, p.split_log2, c, min(32, w.cnt - c), quarter * 32 + lane);
+                            continue;
+                        }
+                        float x[32];
+                        finish_load(c, v, x);
+                        const OutBlock o = block_of(h, c);
+                        if (o.features <= 0) break;  // (uniform) the second half of the last tile along P
+                        if (p.out_type == kOutF32) {
+                            store_block32(x, o, stage_out, quarter, lane, 2 + group);
+                        } else {
+                            uint32_t words[16];
+                            pack_block(x, p.out_type == kOutBF16, words);
+                            store_block16(words, o, stage_out, quarter, lane, 2 + group);
+                        }
+                    }
+                    release(h);
                 }
             }
             if (!empty_sum) acc_phase ^= 1u;
@@ -876,17 +1040,17 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                 }
                 if (p.early) grid_dependency_wait();
                 if (t < per)
-                    red_scale[t] = rank * per + t < w.cnt && !w.zero ? p.scale_q[w.row0 + rank * per + t] : 0.f;
+                    scales[t] = rank * per + t < w.cnt && !w.zero ? p.scale_q[w.row0 + rank * per + t] : 0.f;
             }
         }
         cluster_sync_all();  // every part has arrived
         if (work && t < 256) {
             if (p.out_type == kOutF32)
-                finish<C, float>(p, w, red, red_scale, rank, t, sp, bias);
+                finish<C, float>(p, w, red, scales, rank, t, sp, bias);
             else if (p.out_type == kOutF16)
-                finish<C, __half>(p, w, red, red_scale, rank, t, sp, bias);
+                finish<C, __half>(p, w, red, scales, rank, t, sp, bias);
             else
-                finish<C, __nv_bfloat16>(p, w, red, red_scale, rank, t, sp, bias);
+                finish<C, __nv_bfloat16>(p, w, red, scales, rank, t, sp, bias);
         }
     }
     tc_fence_after();
