@@ -20,13 +20,13 @@ tcg_status fail(cudaError_t e);
 // the driver's tensor-map encoder resolved.
 tcg_status device(int* id, int* sms);
 
-// A 3-D tiled tensor map: extents {d0 (contiguous), d1, d2}, byte strides of
-// d1 and d2, box {box0, box1, 1}.
-struct Box3 {
-    uint64_t d0, d1, d2, s1, s2;
-    uint32_t box0, box1;
+// A 4-D tiled tensor map: extents (innermost first, contiguous), byte strides
+// of the outer three, box extents of the inner three (the fourth is 1).
+struct Box4 {
+    uint64_t d[4], s[3];
+    uint32_t box[3];
 };
-tcg_status encode_3d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, const Box3& b,
+tcg_status encode_4d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, const Box4& b,
                      CUtensorMapSwizzle swz);
 
 bool dependent_launch();               // programmatic dependent launch (TCG_PDL)

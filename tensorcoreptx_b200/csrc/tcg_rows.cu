@@ -4,7 +4,9 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstring>
 
 #include "../../include/tcgemm.h"
@@ -42,41 +44,60 @@ struct RowsPlan {
 
 int ceil_div(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
 
-// Tile and split.  See the measurements in tcg_rows_kernel.cuh.
+// Tile and split: the least of a time model's estimates, in microseconds.  The
+// model is a start (launch, first loads, last stores) plus the k-blocks that
+// the busiest SM works through, each at a measured rate (B200, 36 shapes of
+// 1 to 8192 rows and 1 to 64 groups timed with every tile and split):
+//   kSub = 1:  4.0 + k-blocks x 0.20 (tiles of up to 64 rows: the rate at which
+//              one CTA's loads and MMAs are issued) or x 0.30 (128 rows: bytes
+//              from L2), x tiles per SM
+//   split:     5.5 + the same for a share of the k-blocks.  The exchange costs
+//              1.5; a second wave of clusters costs far more than it saves (48
+//              rows x 10240 x 4096 over 2 CTAs 10.9, over 4 in two waves 14.9),
+//              so all clusters have to be resident at once (two CTAs per SM
+//              with tiles of 16 rows: 16 x 10240 x 4096 8.8 against 10.6
+//              unsplit); clusters of eight CTAs fit few of the GPU's processing clusters (16 of them take
+//              two waves), so at most eight of those.
+//   kSub = 2:  10 + k-blocks x 0.54 (the tensor cores' rate) x whole waves
+// Example: int8 512 x 4096 x 4096 64 rows 13.4 (model 15.1), 128 rows 12.9
+// (13.6), 256 rows 29.1 (27.3); 100 x 4096 x 4096: 32 rows 10.8, 64 rows on two
+// CTAs 9.0, 128 rows on four 8.5.
 RowsPlan choose_plan(const RowsCall& c, bool weight, int kblock, int sms)
 {
     const int forced = g_rows_tile.load(), forced_split = g_rows_split.load();
-    RowsPlan plan{128, 1};
-    const long long mean = (static_cast<long long>(c.rows) + c.groups - 1) / c.groups;  // rows per group
-    long long wide, tiles;
-    if (weight) {
-        wide = static_cast<long long>(c.groups) * ceil_div(c.P, 256) * ceil_div(c.Q, 256);
-    } else {
-        wide = static_cast<long long>(c.groups) * ceil_div(mean, 256) * ceil_div(c.P, 256);
+    const double mean = static_cast<double>(c.rows) / c.groups;  // rows per group
+    const double kb = weight ? (mean + kblock - 1) / kblock : ceil_div(c.R, kblock);
+    const double used = c.groups < c.rows ? c.groups : c.rows;   // groups that can have rows
+    RowsPlan best{128, 1};
+    double least = -1;
+    for (int bq = weight ? 128 : 16; bq <= 256; bq *= 2) {
+        if (forced && bq != forced && !(weight && forced < 128 && bq == 128)) continue;
+        const int tile_p = bq == 256 ? 256 : 128;
+        double q;  // tiles along q: a ragged group ends half a tile early on average
+        if (weight)
+            q = static_cast<double>(c.groups) * ceil_div(c.Q, bq);
+        else if (!c.offsets)
+            q = static_cast<double>(c.groups) * ceil_div(c.rows / c.groups, bq);
+        else
+            q = std::max(used, static_cast<double>(c.rows) / bq + 0.5 * used);
+        const double tiles = q * ceil_div(c.P, tile_p);
+        for (int split = 1; split <= (bq == 256 ? 1 : 8); split *= 2) {
+            if (forced_split && bq != 256 && split != forced_split) continue;
+            const bool resident = split == 8 ? tiles <= 8 : tiles * split <= (bq == 16 ? 2 : 1) * sms;
+            if (split > 1 && !resident && !forced_split) continue;
+            double t;
+            if (bq == 256)
+                t = 10.0 + std::ceil(tiles / sms) * kb * 0.54;
+            else
+                t = (split > 1 ? 5.5 : 4.0) +
+                    std::max(1.0, tiles * split / sms) * kb / split * (bq == 128 ? 0.30 : 0.20);
+            if (least < 0 || t < least) {
+                least = t;
+                best = RowsPlan{bq, split};
+            }
+        }
     }
-    if (forced) {
-        plan.bq = forced;
-        if (weight && plan.bq < 128) plan.bq = 128;
-    } else if ((weight || mean > 96) && 4 * wide >= 3 * sms) {
-        plan.bq = 256;
-    } else if (!weight) {
-        plan.bq = 16;
-        while (plan.bq < 128 && 4 * plan.bq < 5 * mean) plan.bq *= 2;
-        if (!c.offsets && plan.bq > 16 && plan.bq / 2 >= mean) plan.bq /= 2;
-    }
-    if (plan.bq == 256) return plan;
-    if (weight)
-        tiles = static_cast<long long>(c.groups) * ceil_div(c.P, 128) * ceil_div(c.Q, plan.bq);
-    else
-        tiles = static_cast<long long>(c.groups < c.rows ? c.groups : c.rows) * ceil_div(mean, plan.bq) *
-                ceil_div(c.P, 128);
-    const long long kb = ceil_div(weight ? mean : c.R, kblock);
-    if (forced_split) {
-        plan.split = forced_split;
-    } else {
-        while (plan.split < 8 && tiles * plan.split * 2 <= 2LL * sms && kb >= 8LL * plan.split) plan.split *= 2;
-    }
-    return plan;
+    return best;
 }
 
 template <class C>
@@ -95,21 +116,37 @@ tcg_status launch(const RowsCall& c, int split, int dev, int sms, cudaStream_t s
     const CUtensorMapDataType dt = C::kElem == 2 ? t16 : t8;
     const uint64_t es = C::kElem, P = c.P, Q = c.Q, R = c.R, M = c.rows, G = c.groups;
     const CUtensorMapSwizzle swz = CU_TENSOR_MAP_SWIZZLE_128B;
-    CUtensorMap mp, mq;
+    // An MN-major operand of whole 64-element atoms is seen as {64, rows, atoms,
+    // groups}, so that one copy brings a tile's atoms; otherwise (the last atom
+    // ends inside a row) as {elements, rows, 1, groups}, a copy per atom.
+    const uint32_t bk = C::kBK;
+    const bool p_whole = c.P % 64 == 0, q_whole = c.Q % 64 == 0;
+    const auto atoms = [&](uint64_t width, uint64_t rows, uint64_t groups, bool whole, uint32_t n) {
+        const uint64_t pitch = width * es;
+        return whole ? host::Box4{{64, rows, width / 64, groups}, {pitch, 128, rows * pitch}, {64, bk, n}}
+                     : host::Box4{{width, rows, 1, groups}, {pitch, rows * pitch, rows * pitch}, {64, bk, 1}};
+    };
+    const auto k_major = [&](uint64_t rows, uint64_t groups, uint32_t n) {
+        const uint64_t pitch = R * es;
+        return host::Box4{{R, rows, 1, groups}, {pitch, rows * pitch, rows * pitch}, {bk, n, 1}};
+    };
+    CUtensorMap mp, mq, mqb;  // mqb: rows in boxes of kQBox, for tiles that are not full
     tcg_status s;
     if (C::kConv)
-        s = host::encode_3d(&mp, t8, c.pside, {P, M, 1, P, M * P, 128, C::kBK}, CU_TENSOR_MAP_SWIZZLE_NONE);
+        s = host::encode_4d(&mp, t8, c.pside, {{P, M, 1, 1}, {P, M * P, M * P}, {C::kTileP, bk, 1}},
+                            CU_TENSOR_MAP_SWIZZLE_NONE);
     else if (C::kWeight)
-        s = host::encode_3d(&mp, dt, c.pside, {P, M, 1, P * es, M * P * es, 64, C::kBK}, swz);
+        s = host::encode_4d(&mp, dt, c.pside, atoms(P, M, 1, p_whole, 2 * C::kSub), swz);
     else if (C::kPMn)
-        s = host::encode_3d(&mp, dt, c.pside, {P, R, G, P * es, R * P * es, 64, C::kBK}, swz);
+        s = host::encode_4d(&mp, dt, c.pside, atoms(P, R, G, p_whole, 2 * C::kSub), swz);
     else
-        s = host::encode_3d(&mp, dt, c.pside, {R, P, G, R * es, P * R * es, C::kBK, 128}, swz);
-    if (s != TCG_SUCCESS) return s;
-    if (C::kWeight)
-        s = host::encode_3d(&mq, dt, c.qside, {Q, M, 1, Q * es, M * Q * es, 64, C::kBK}, swz);
-    else
-        s = host::encode_3d(&mq, dt, c.qside, {R, M, 1, R * es, M * R * es, C::kBK, C::kQBox}, swz);
+        s = host::encode_4d(&mp, dt, c.pside, k_major(P, G, C::kTileP), swz);
+    if (s == TCG_SUCCESS)
+        s = C::kWeight ? host::encode_4d(&mq, dt, c.qside, atoms(Q, M, 1, q_whole, C::kBQ / 64), swz)
+                       : host::encode_4d(&mq, dt, c.qside, k_major(M, 1, C::kBQ), swz);
+    mqb = mq;
+    if (s == TCG_SUCCESS && !C::kWeight && C::kBQ > C::kQBox)
+        s = host::encode_4d(&mqb, dt, c.qside, k_major(M, 1, C::kQBox), swz);
     if (s != TCG_SUCCESS) return s;
 
     RowsParams p;
@@ -136,6 +173,8 @@ tcg_status launch(const RowsCall& c, int split, int dev, int sms, cudaStream_t s
     p.bf16 = c.bf16;
     while ((1 << p.split_log2) < split) ++p.split_log2;
     p.early = c.early;
+    p.p_whole = p_whole;
+    p.q_whole = q_whole;
     const int table = c.offsets ? c.groups : 0;
     const uint32_t fmt = C::kKind == kKindI8 ? 1u : (c.bf16 ? 1u : 0u);
     p.idesc = make_idesc(C::kKind == kKindI8 ? 2u : 1u, fmt, fmt, C::kQMn, 128, 0) | (C::kPMn ? 1u << 15 : 0u);
@@ -190,7 +229,7 @@ tcg_status launch(const RowsCall& c, int split, int dev, int sms, cudaStream_t s
         attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
         ++cfg.numAttrs;
     }
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, mp, mq, p);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, mp, mq, mqb, p);
     return e == cudaSuccess ? TCG_SUCCESS : host::fail(e);
 }
 

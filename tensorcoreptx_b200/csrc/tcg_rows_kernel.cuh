@@ -64,6 +64,7 @@ struct RowsParams {
     int bf16;                 // 16-bit operands are bf16 (kConv: type of the widened codes)
     int split_log2;           // kSub = 1: 1, 2, 4 or 8 CTAs per tile
     int stages;               // ring depth
+    int p_whole, q_whole;     // MN-major operands of whole 64-element atoms: one copy a tile and stage
     int early;                // the M-side operand and the offsets predate the kernel this one follows
     uint32_t idesc;           // instruction descriptor without N
 };
@@ -75,17 +76,20 @@ struct RowsTraits {
     static constexpr int kSub = kSub_, kBQ = kBQ_;
     static constexpr bool kWeight = kQMn;               // weight form: the sum runs over a group's rows
     static constexpr int kElem = kKind == kKindF16 ? 2 : 1;
-    static constexpr int kBK = 128 / kElem;             // length of the sum per ring stage
+    // length of the sum per ring stage; kConv: a quarter of a row of codes, so that
+    // stages are small and many enough to hide the conversion
+    static constexpr int kBK = kConv ? 32 : 128 / kElem;
     static constexpr int kUmmaK = 32 / kElem;
     static constexpr int kTileP = 128 * kSub;
-    static constexpr int kSubBytes = 128 * 128;         // one 128-feature block of a stage
+    static constexpr int kSubBytes = 128 * kBK * kElem; // one 128-feature block of a stage
     static constexpr int kPBytes = kSub * kSubBytes;
-    static constexpr int kQBytes = kBQ * 128;
-    static constexpr int kStageBytes = kPBytes + kQBytes;
-    static constexpr int kQBox = kBQ < 64 ? kBQ : 64;   // rows (weight form: columns) per box of the q operand
-    static constexpr int kQBoxBytes = kQBox * 128;
+    static constexpr int kQBytes = kBQ * kBK * kElem;
     static constexpr int kRawBytes = 128 * kBK;         // kConv: int8 codes of one 128-feature block
-    static constexpr int kConvWarps = kConv ? 8 : 0;
+    static constexpr int kStageBytes = kPBytes + kQBytes + (kConv ? kSub * kRawBytes : 0);
+    static constexpr int kAtomBytes = 128 * kBK;        // MN-major: 64 elements of kBK rows
+    static constexpr int kQBox = kBQ < 64 ? kBQ : 64;   // rows (weight form: columns) per box of the q operand
+    static constexpr int kQBoxBytes = kQBox * kBK * kElem;
+    static constexpr int kConvWarps = kConv ? 8 : 0;    // two groups of four, taking stages in turn
     static constexpr int kEpiWarps = 8;                 // two per quarter of the tensor memory's lanes
     static constexpr int kFirstConv = 2 + kEpiWarps;
     static constexpr int kThreads = 32 * (kFirstConv + kConvWarps);
@@ -297,47 +301,40 @@ __device__ __forceinline__ void store_block16(const uint32_t (&w)[16], const Out
     for (int j = 0; j < 16; ++j) stage[j * 128 + quarter * 32 + lane] = w[j];
     group_sync(barrier);
     unsigned short* out = static_cast<unsigned short*>(o.out) + o.row * o.ld + o.f;
-    if (o.aligned) {
-        // 16 lanes a row pair, eight features a lane
-        const int e = (lane & 15) * 8;
+    const int e = (lane & 15) * 8;  // 16 lanes a row pair, eight features a lane
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int pair = quarter * 4 + i * 2 + (lane >> 4);
-            const uint4 a = *reinterpret_cast<const uint4*>(stage + pair * 128 + e);
-            const uint4 b = *reinterpret_cast<const uint4*>(stage + pair * 128 + e + 4);
-            unsigned short* row = out + static_cast<long long>(2 * pair) * o.ld + e;
-            if (e < o.features && 2 * pair < o.n)
-                *reinterpret_cast<uint4*>(row) =
-                    make_uint4(__byte_perm(a.x, a.y, 0x5410), __byte_perm(a.z, a.w, 0x5410),
-                               __byte_perm(b.x, b.y, 0x5410), __byte_perm(b.z, b.w, 0x5410));
-            if (e < o.features && 2 * pair + 1 < o.n)
-                *reinterpret_cast<uint4*>(row + o.ld) =
-                    make_uint4(__byte_perm(a.x, a.y, 0x7632), __byte_perm(a.z, a.w, 0x7632),
-                               __byte_perm(b.x, b.y, 0x7632), __byte_perm(b.z, b.w, 0x7632));
-        }
-    } else {
-        // rows of odd length: aligned words of two features, and single ones at the ends
-#pragma unroll 1
-        for (int i = 0; i < 8; ++i) {
-            const int r = quarter * 8 + i;
-            if (r >= o.n) break;
-            unsigned short* row = out + static_cast<long long>(r) * o.ld;
-            const uint32_t* line = stage + (r >> 1) * 128;
-            const int shift = (r & 1) * 16;
-            const int odd = static_cast<int>(reinterpret_cast<uintptr_t>(row) >> 1) & 1;
-            if (odd && lane == 0) row[0] = static_cast<unsigned short>(line[0] >> shift);
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int e = 2 * (lane + 32 * u) + odd;
-                if (e + 1 < o.features)
-                    *reinterpret_cast<uint32_t*>(row + e) =
-                        __byte_perm(line[e], line[e + 1], shift ? 0x7632 : 0x5410);
-                else if (e < o.features)
-                    row[e] = static_cast<unsigned short>(line[e] >> shift);
-            }
-        }
+    for (int i = 0; i < 2; ++i) {
+        const int pair = quarter * 4 + i * 2 + (lane >> 4);
+        const uint4 a = *reinterpret_cast<const uint4*>(stage + pair * 128 + e);
+        const uint4 b = *reinterpret_cast<const uint4*>(stage + pair * 128 + e + 4);
+        unsigned short* row = out + static_cast<long long>(2 * pair) * o.ld + e;
+        if (e < o.features && 2 * pair < o.n)
+            *reinterpret_cast<uint4*>(row) =
+                make_uint4(__byte_perm(a.x, a.y, 0x5410), __byte_perm(a.z, a.w, 0x5410),
+                           __byte_perm(b.x, b.y, 0x5410), __byte_perm(b.z, b.w, 0x5410));
+        if (e < o.features && 2 * pair + 1 < o.n)
+            *reinterpret_cast<uint4*>(row + o.ld) =
+                make_uint4(__byte_perm(a.x, a.y, 0x7632), __byte_perm(a.z, a.w, 0x7632),
+                           __byte_perm(b.x, b.y, 0x7632), __byte_perm(b.z, b.w, 0x7632));
     }
     group_sync(barrier);
+}
+
+// Rows that are not whole 16-byte vectors: straight from the registers, 64
+// bytes of a row per warp and store.  (Putting rows of odd length together
+// from aligned words in shared memory measured slower: int8 1777 x 4099 x 4096
+// 38 against 29 us.)
+__device__ __forceinline__ void store_rows16(const uint32_t (&w)[16], const OutBlock& o, int quarter, int lane)
+{
+    const int e = quarter * 32 + lane;
+    const bool live = e < o.features;
+    unsigned short* ptr = static_cast<unsigned short*>(o.out) + o.row * o.ld + o.f + e;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        if (2 * j < o.n && live) ptr[0] = static_cast<unsigned short>(w[j]);
+        if (2 * j + 1 < o.n && live) ptr[o.ld] = static_cast<unsigned short>(w[j] >> 16);
+        ptr += 2 * static_cast<long long>(o.ld);
+    }
 }
 
 __device__ __forceinline__ void store_block32(const float (&x)[32], const OutBlock& o, uint32_t* stage, int quarter,
@@ -368,32 +365,50 @@ __device__ __forceinline__ void store_block32(const float (&x)[32], const OutBlo
     }
 }
 
-// kConv: one ring stage of int8 codes (64 rows x 128 features per block, rows
-// of 128 bytes) into 16-bit values code * scale[row] in the MN-major
+// kConv: one ring stage of int8 codes (kBK rows of the tile's features) into 16-bit values code * scale[row] in the MN-major
 // 128-byte-swizzled layout the MMA reads: per block two atoms of 64 features,
 // an atom's row r at r * 128 with its 16-byte chunk c at c ^ (r & 7).  The
 // product of code and scale is rounded to 16 bits: at most half a step of
 // the operand type, against half a code step (2^-8 of the row's largest value)
 // that the codes themselves are off by.
-// In place: the codes land in the upper half of the stage's P area; each
-// thread takes its codes into registers, and after a barrier of the converter
-// warps writes them widened.  Eight consecutive threads hold one row; threads
-// 4..7 write their two chunks in the other order, so the eight chunks of a
-// write lie in different banks.
+// The codes have an area of their own in the stage, so that no thread waits for
+// another before it writes (in place, with a barrier between reading and
+// writing, a stage took 300 cycles longer).  Eight consecutive threads hold one
+// row.  Rows past the end of the group have scale 0 and become zeros.  The
+// integer pipe bounds this: per four codes one exclusive-or, four byte
+// permutes and two packs at two cycles a warp each.
+constexpr int kConvThreads = 128;
+constexpr int kConvRows = kConvThreads / 8;  // rows of one block per pass
+
 template <class C>
 struct ConvRegs {
-    uint4 v[2 * C::kSub];
-    float s[2 * C::kSub];
+    static constexpr int kPerBlock = C::kBK / kConvRows;
+    uint4 v[kPerBlock * C::kSub];
+    float s[kPerBlock];
 };
 
-// codes of one thread: pass u is 16 codes of row (u & 1) * 32 + ct / 8 of block u / 2
+// scales of one thread's rows of the k-block that starts at row r0 (rend: end of the group)
+template <class C>
+__device__ __forceinline__ void conv_scales(const RowsParams& p, int r0, int rend, int ct,
+                                            float (&s)[ConvRegs<C>::kPerBlock])
+{
+#pragma unroll
+    for (int u = 0; u < ConvRegs<C>::kPerBlock; ++u) {
+        const int r = r0 + u * kConvRows + (ct >> 3);
+        s[u] = r < rend ? p.scale_r[r] : 0.f;
+    }
+}
+
+// pass u of block b is 16 codes of row u * kConvRows + ct / 8
 template <class C>
 __device__ __forceinline__ void conv_codes(const uint8_t* raw, int ct, ConvRegs<C>& g)
 {
 #pragma unroll
-    for (int u = 0; u < 2 * C::kSub; ++u)
-        g.v[u] = *reinterpret_cast<const uint4*>(raw + (u >> 1) * C::kRawBytes + ((u & 1) * 32 + (ct >> 3)) * 128 +
-                                                 (ct & 7) * 16);
+    for (int b = 0; b < C::kSub; ++b)
+#pragma unroll
+        for (int u = 0; u < g.kPerBlock; ++u)
+            g.v[b * g.kPerBlock + u] = *reinterpret_cast<const uint4*>(
+                raw + (u * kConvRows + (ct >> 3)) * C::kTileP + b * 128 + (ct & 7) * 16);
 }
 
 __device__ __forceinline__ float code_float(uint32_t w, int i)
@@ -403,27 +418,28 @@ __device__ __forceinline__ float code_float(uint32_t w, int i)
 }
 
 template <class C, bool kBf16>
-__device__ __forceinline__ void conv_write(uint8_t* p_area, int ct, int valid, const ConvRegs<C>& g)
+__device__ __forceinline__ void conv_write(uint8_t* p_area, int ct, const ConvRegs<C>& g)
 {
     const int c = ct & 7;
 #pragma unroll
-    for (int u = 0; u < 2 * C::kSub; ++u) {
-        const int r = (u & 1) * 32 + (ct >> 3);
-        uint4 o[2];
-        uint32_t* ow = reinterpret_cast<uint32_t*>(o);
-        const uint32_t in[4] = {g.v[u].x ^ 0x80808080u, g.v[u].y ^ 0x80808080u, g.v[u].z ^ 0x80808080u,
-                                g.v[u].w ^ 0x80808080u};
+    for (int b = 0; b < C::kSub; ++b)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            ow[2 * i] = pack16<kBf16>(code_float(in[i], 0) * g.s[u], code_float(in[i], 1) * g.s[u]);
-            ow[2 * i + 1] = pack16<kBf16>(code_float(in[i], 2) * g.s[u], code_float(in[i], 3) * g.s[u]);
+        for (int u = 0; u < g.kPerBlock; ++u) {
+            const int r = u * kConvRows + (ct >> 3);
+            const uint4 v = g.v[b * g.kPerBlock + u];
+            const float s = g.s[u];
+            uint4 o[2];
+            uint32_t* ow = reinterpret_cast<uint32_t*>(o);
+            const uint32_t in[4] = {v.x ^ 0x80808080u, v.y ^ 0x80808080u, v.z ^ 0x80808080u, v.w ^ 0x80808080u};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                ow[2 * i] = pack16<kBf16>(code_float(in[i], 0) * s, code_float(in[i], 1) * s);
+                ow[2 * i + 1] = pack16<kBf16>(code_float(in[i], 2) * s, code_float(in[i], 3) * s);
+            }
+            uint8_t* row = p_area + b * C::kSubBytes + (c >> 2) * C::kAtomBytes + r * 128;
+            *reinterpret_cast<uint4*>(row + (((2 * (c & 3)) ^ (r & 7)) << 4)) = o[0];
+            *reinterpret_cast<uint4*>(row + (((2 * (c & 3) + 1) ^ (r & 7)) << 4)) = o[1];
         }
-        if (r >= valid) o[0] = o[1] = make_uint4(0, 0, 0, 0);  // rows of the next group
-        uint8_t* row = p_area + (u >> 1) * C::kSubBytes + (c >> 2) * 8192 + r * 128;
-        const int first = c >> 2;
-        *reinterpret_cast<uint4*>(row + (((2 * (c & 3) + first) ^ (r & 7)) << 4)) = first ? o[1] : o[0];
-        *reinterpret_cast<uint4*>(row + (((2 * (c & 3) + (first ^ 1)) ^ (r & 7)) << 4)) = first ? o[0] : o[1];
-    }
 }
 
 // Split sums.  Columns c .. c + n - 1 of this CTA's part (one lane = feature
@@ -506,7 +522,7 @@ __device__ __forceinline__ void finish(const RowsParams& p, const RowsItem& w, c
 template <class C>
 __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
     rows_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ CUtensorMap tmQ,
-                const __grid_constant__ RowsParams p)
+                const __grid_constant__ CUtensorMap tmQb, const __grid_constant__ RowsParams p)
 {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -536,7 +552,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
         if (lane < stages) {
             mbar_init(smem_u32(&full[lane]), 1);
             mbar_init(smem_u32(&empty[lane]), 1);
-            if (C::kConv) mbar_init(smem_u32(&conv[lane]), C::kConvWarps);
+            if (C::kConv) mbar_init(smem_u32(&conv[lane]), C::kConvWarps / 2);
         } else if (lane >= 16 && lane < 18) {
             mbar_init(smem_u32(&tfull[lane - 16]), 1);
             mbar_init(smem_u32(&tempty[lane - 16]), C::kEpiWarps);
@@ -547,6 +563,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
             tma_prefetch_desc(&tmP);
         } else if (lane == 20) {
             tma_prefetch_desc(&tmQ);
+        } else if (lane == 21) {
+            tma_prefetch_desc(&tmQb);
         }
         fence_mbar_init();
     }
@@ -599,29 +617,39 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
         int stage = 0;
         uint32_t phase = 0;
         bool aborted = false;
+        // One copy per operand and stage wherever the layout allows: a copy costs
+        // this thread about 100 cycles, and eight of them per stage bounded the
+        // MN-major products.
         const auto load_p = [&](const RowsItem& w, int kb, int st, int blocks) {
             const uint32_t dst = ring + st * C::kStageBytes, fb = smem_u32(&full[st]);
-            for (int h = 0; h < blocks; ++h) {
-                const int f = w.p0 + h * 128;
-                if constexpr (C::kConv) {
-                    tma_load_3d(dst + C::kSub * C::kRawBytes + h * C::kRawBytes, &tmP, fb, f, w.row0 + kb * C::kBK, 0);
-                } else if constexpr (C::kPMn) {
-                    const int r = C::kWeight ? w.row0 + kb * C::kBK : kb * C::kBK;
-                    const int z = C::kWeight ? 0 : w.e;
-                    tma_load_3d(dst + h * C::kSubBytes, &tmP, fb, f, r, z);
-                    tma_load_3d(dst + h * C::kSubBytes + 8192, &tmP, fb, f + 64, r, z);
-                } else {
-                    tma_load_3d(dst + h * C::kSubBytes, &tmP, fb, kb * C::kBK, f, w.e);
-                }
+            if constexpr (C::kConv) {
+                tma_load_4d(dst + C::kPBytes + C::kQBytes, &tmP, fb, w.p0, w.row0 + kb * C::kBK, 0, 0);
+            } else if constexpr (C::kPMn) {
+                const int r = C::kWeight ? w.row0 + kb * C::kBK : kb * C::kBK;
+                const int z = C::kWeight ? 0 : w.e;
+                if (p.p_whole)
+                    tma_load_4d(dst, &tmP, fb, 0, r, w.p0 / 64, z);
+                else
+                    for (int a = 0; a < 2 * blocks; ++a)
+                        tma_load_4d(dst + a * C::kAtomBytes, &tmP, fb, w.p0 + a * 64, r, 0, z);
+            } else {
+                tma_load_4d(dst, &tmP, fb, kb * C::kBK, w.p0, 0, w.e);
             }
         };
         const auto load_q = [&](const RowsItem& w, int kb, int st, int boxes) {
             const uint32_t dst = ring + st * C::kStageBytes + C::kPBytes, fb = smem_u32(&full[st]);
-            for (int b = 0; b < boxes; ++b) {
-                if constexpr (C::kQMn)
-                    tma_load_3d(dst + b * C::kQBoxBytes, &tmQ, fb, w.q0 + b * 64, w.row0 + kb * C::kBK, 0);
+            if constexpr (C::kQMn) {
+                if (p.q_whole)
+                    tma_load_4d(dst, &tmQ, fb, 0, w.row0 + kb * C::kBK, w.q0 / 64, 0);
                 else
-                    tma_load_3d(dst + b * C::kQBoxBytes, &tmQ, fb, kb * C::kBK, w.row0 + b * C::kQBox, 0);
+                    for (int b = 0; b < boxes; ++b)
+                        tma_load_4d(dst + b * C::kAtomBytes, &tmQ, fb, w.q0 + b * 64, w.row0 + kb * C::kBK, 0, 0);
+            } else {
+                if (boxes * C::kQBox == C::kBQ)
+                    tma_load_4d(dst, &tmQ, fb, kb * C::kBK, w.row0, 0, 0);
+                else
+                    for (int b = 0; b < boxes; ++b)
+                        tma_load_4d(dst + b * C::kQBoxBytes, &tmQb, fb, kb * C::kBK, w.row0 + b * C::kQBox, 0, 0);
             }
         };
         bool waited = !p.early;
@@ -631,8 +659,10 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
             share(w, kb0, kb1);
             const int blocks = blocks_of(w);
             const int boxes = (w.cnt + C::kQBox - 1) / C::kQBox;
-            const uint32_t tx = static_cast<uint32_t>(blocks * (C::kConv ? C::kRawBytes : C::kSubBytes) +
-                                                      boxes * C::kQBoxBytes);
+            const int p_bytes = C::kConv ? C::kSub * C::kRawBytes
+                                         : (C::kPMn && !p.p_whole ? blocks * C::kSubBytes : C::kPBytes);
+            const int q_bytes = C::kQMn && p.q_whole ? C::kQBytes : boxes * C::kQBoxBytes;
+            const uint32_t tx = static_cast<uint32_t>(p_bytes + q_bytes);
             int kb = kb0;
             if (!waited) {
                 // the first ring-full: features now, rows once the kernel before has finished
@@ -681,8 +711,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
         uint32_t phase = 0;
         uint32_t acc_phase = 0;
         bool aborted = false;
-        const uint64_t pdesc = C::kPMn ? smem_desc_sw128(ring, 8192, 1024) : smem_desc_sw128(ring, 16, 1024);
-        const uint64_t qdesc = C::kQMn ? smem_desc_sw128(ring + C::kPBytes, 8192, 1024)
+        const uint64_t pdesc = C::kPMn ? smem_desc_sw128(ring, C::kAtomBytes, 1024) : smem_desc_sw128(ring, 16, 1024);
+        const uint64_t qdesc = C::kQMn ? smem_desc_sw128(ring + C::kPBytes, C::kAtomBytes, 1024)
                                        : smem_desc_sw128(ring + C::kPBytes, 16, 1024);
         for (int item = first; item < total && !aborted; item += stride) {
             const RowsItem w = tile_of(item);
@@ -711,7 +741,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                 const int pa = C::kConv ? 0 : 2 * blocks;
                 for (int i = lane; i < (pa + (n + 63) / 64) * extra * 8; i += 32) {
                     const int a = i / (extra * 8), r = valid + (i / 8) % extra;
-                    uint8_t* atom = a < pa ? base + a * 8192 : base + C::kPBytes + (a - pa) * 8192;
+                    uint8_t* atom = base + (a < pa ? a * C::kAtomBytes : C::kPBytes + (a - pa) * C::kAtomBytes);
                     *reinterpret_cast<uint4*>(atom + r * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
                 }
                 fence_proxy_async_smem();
@@ -933,7 +963,12 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                     for (int i = 0; i < 4; ++i) {
                         const int c = 32 * group + 64 * i;
                         const OutBlock o = block_of(h, c);
-                        if (c < w.cnt && o.features > 0) store_block16(held[h][i], o, stage_out, quarter, lane, 2 + group);
+                        if (c < w.cnt && o.features > 0) {
+                            if (o.aligned)
+                                store_block16(held[h][i], o, stage_out, quarter, lane, 2 + group);
+                            else
+                                store_rows16(held[h][i], o, quarter, lane);
+                        }
                     }
             } else {
                 for (int h = 0; h < C::kSub; ++h) {
@@ -957,7 +992,10 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                         } else {
                             uint32_t words[16];
                             pack_block(x, p.out_type == kOutBF16, words);
-                            store_block16(words, o, stage_out, quarter, lane, 2 + group);
+                            if (o.aligned)
+                                store_block16(words, o, stage_out, quarter, lane, 2 + group);
+                            else
+                                store_rows16(words, o, quarter, lane);
                         }
                     }
                     release(h);
@@ -967,39 +1005,39 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
         }
     } else if (C::kConv && warp >= C::kFirstConv) {
         // -------------------------------------------------- converters ----
-        // Every wait's outcome goes through a barrier-AND of the converter
-        // warps, so they give up together.
-        const int ct = static_cast<int>(threadIdx.x) - 32 * C::kFirstConv;
-        int stage = 0;
+        const int conv_group = (warp - C::kFirstConv) >> 2;
+        const int ct = (static_cast<int>(threadIdx.x) - 32 * C::kFirstConv) & (kConvThreads - 1);
+        int stage = 0, turn = 0;
         uint32_t phase = 0;
         bool ok = true;
         for (int item = first; item < total && ok; item += stride) {
             const RowsItem w = tile_of(item);
             int kb0, kb1;
             share(w, kb0, kb1);
-            for (int kb = kb0; kb < kb1; ++kb) {
-                ConvRegs<C> g;
-                const int valid = valid_of(w, kb);
+            // the scales are fetched a turn ahead: their latency is several conversions long
+            float ahead[ConvRegs<C>::kPerBlock];
+            conv_scales<C>(p, w.row0 + (kb0 + (turn ^ conv_group)) * C::kBK, w.rend, ct, ahead);
+            for (int kb = kb0; kb < kb1; ++kb, turn ^= 1) {
+                if (turn == conv_group) {
+                    ConvRegs<C> g;
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int r = u * 32 + (ct >> 3);
-                    const float s = r < valid ? p.scale_r[w.row0 + kb * C::kBK + r] : 0.f;
-#pragma unroll
-                    for (int b = 0; b < C::kSub; ++b) g.s[2 * b + u] = s;
+                    for (int u = 0; u < g.kPerBlock; ++u) g.s[u] = ahead[u];
+                    conv_scales<C>(p, w.row0 + (kb + 2) * C::kBK, w.rend, ct, ahead);
+                    if (!wait_bounded_warp(smem_u32(&full[stage]), phase, abort_flag, p.timeout_ns,
+                                           (blockIdx.x << 8) | 0xA0u | stage)) {
+                        ok = false;
+                        break;
+                    }
+                    uint8_t* st = smem + stage * C::kStageBytes;
+                    conv_codes<C>(st + C::kPBytes + C::kQBytes, ct, g);
+                    if (p.bf16)
+                        conv_write<C, true>(st, ct, g);
+                    else
+                        conv_write<C, false>(st, ct, g);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&conv[stage]));
                 }
-                const bool landed = wait_bounded_warp(smem_u32(&full[stage]), phase, abort_flag, p.timeout_ns,
-                                                      (blockIdx.x << 8) | 0xA0u | stage);
-                uint8_t* st = smem + stage * C::kStageBytes;
-                if (landed) conv_codes<C>(st + C::kSub * C::kRawBytes, ct, g);
-                ok = named_barrier_and(1, 32 * C::kConvWarps, landed);
-                if (!ok) break;
-                if (p.bf16)
-                    conv_write<C, true>(st, ct, valid, g);
-                else
-                    conv_write<C, false>(st, ct, valid, g);
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&conv[stage]));
                 if (++stage == stages) stage = 0, phase ^= 1u;
             }
         }

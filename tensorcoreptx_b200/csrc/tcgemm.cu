@@ -139,17 +139,14 @@ tcg_status encode_3d(CUtensorMap* map, CUtensorMapDataType dt, const void* base,
     return s;
 }
 
-tcg_status encode_3d_uncached(CUtensorMap* map, CUtensorMapDataType dt, const void* base, uint64_t d0, uint64_t d1,
-                              uint64_t d2, uint64_t s1, uint64_t s2, uint32_t box0, uint32_t box1,
-                              CUtensorMapSwizzle swz)
+tcg_status encode_tiled(CUtensorMap* map, CUtensorMapDataType dt, int rank, const void* base, const cuuint64_t* dims,
+                        const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swz)
 {
-    cuuint64_t dims[3] = {d0, d1, d2};
-    cuuint64_t strides[2] = {s1, s2};
-    cuuint32_t box[3] = {box0, box1, 1};
-    cuuint32_t estr[3] = {1, 1, 1};
+    const cuuint32_t estr[4] = {1, 1, 1, 1};
     const auto encode = [&]() {
-        return g_encode(map, dt, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        swz, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        return g_encode(map, dt, rank, const_cast<void*>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, swz, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     };
     CUresult r = encode();
     if (r == CUDA_ERROR_INVALID_CONTEXT) {
@@ -163,6 +160,16 @@ tcg_status encode_3d_uncached(CUtensorMap* map, CUtensorMapDataType dt, const vo
         return TCG_ERR_CUDA;
     }
     return TCG_SUCCESS;
+}
+
+tcg_status encode_3d_uncached(CUtensorMap* map, CUtensorMapDataType dt, const void* base, uint64_t d0, uint64_t d1,
+                              uint64_t d2, uint64_t s1, uint64_t s2, uint32_t box0, uint32_t box1,
+                              CUtensorMapSwizzle swz)
+{
+    const cuuint64_t dims[3] = {d0, d1, d2};
+    const cuuint64_t strides[2] = {s1, s2};
+    const cuuint32_t box[3] = {box0, box1, 1};
+    return encode_tiled(map, dt, 3, base, dims, strides, box, swz);
 }
 
 // Tile shape.  Problems that fill a wave of SM pairs with 512 x 256 tiles
@@ -614,10 +621,13 @@ tcg_status device(int* id, int* sms)
     return resolve_encode();
 }
 
-tcg_status encode_3d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, const Box3& b,
+tcg_status encode_4d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, const Box4& b,
                      CUtensorMapSwizzle swz)
 {
-    return encode_3d_uncached(map, dt, base, b.d0, b.d1, b.d2, b.s1, b.s2, b.box0, b.box1, swz);
+    const cuuint64_t dims[4] = {b.d[0], b.d[1], b.d[2], b.d[3]};
+    const cuuint64_t strides[3] = {b.s[0], b.s[1], b.s[2]};
+    const cuuint32_t box[4] = {b.box[0], b.box[1], b.box[2], 1};
+    return encode_tiled(map, dt, 4, base, dims, strides, box, swz);
 }
 
 bool dependent_launch() { return pdl_enabled(); }

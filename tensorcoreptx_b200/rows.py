@@ -30,7 +30,12 @@ from .gemm import _check, _stream_ptr
 
 _TYPES = {torch.float32: nat.TCG_F32, torch.float16: nat.TCG_F16, torch.bfloat16: nat.TCG_BF16}
 _HALVES = (torch.float16, torch.bfloat16)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
+
+# Small calls are bound by the host, so what every call passes through stays
+# short: checks build their message only when they fail, and results are made
+# with Tensor.new_empty / empty_like (a third of torch.empty's time here).
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
@@ -39,42 +44,45 @@ def _ptr(t):
 def _call(fn: str, like: torch.Tensor, *args):
     """nat.lib().<fn>(*args, stream) on like's device and its current stream."""
     f = getattr(nat.lib(), fn)
-    if torch.cuda.current_device() == like.get_device():
+    if _current_device() == like.get_device():
         st = f(*args, _stream_ptr(like))
     else:
         with torch.cuda.device(like.device):
             st = f(*args, _stream_ptr(like))
-    nat.check(fn, st)
+    if st != nat.TCG_SUCCESS:
+        nat.check(fn, st)
 
 
-def _same_device(first, **others):
-    for name, t in others.items():
-        _check(t is None or t.device == first.device, f"{name} must be on the same device as the other operands")
+def _same_device(like, name, t):
+    if t is not None and t.get_device() != like.get_device():
+        raise RuntimeError(f"{name} must be on the same device as the other operands")
 
 
 def _check_offsets(offsets, groups: int, like):
-    _check(offsets.is_cuda and offsets.dtype == torch.int32 and offsets.dim() == 1 and offsets.is_contiguous(),
-           "offsets must be a contiguous 1-D CUDA int32 tensor")
+    if not (offsets.is_cuda and offsets.dtype == torch.int32 and offsets.dim() == 1 and offsets.is_contiguous()):
+        raise RuntimeError("offsets must be a contiguous 1-D CUDA int32 tensor")
     _check(offsets.numel() == groups + 1, "offsets must have one entry more than there are groups")
-    _check(0 < groups <= nat.TCG_MAX_GROUPS, f"the number of groups must be 1 to {nat.TCG_MAX_GROUPS}")
-    _same_device(like, offsets=offsets)
+    if not 0 < groups <= nat.TCG_MAX_GROUPS:
+        raise RuntimeError(f"the number of groups must be 1 to {nat.TCG_MAX_GROUPS}")
+    _same_device(like, "offsets", offsets)
 
 
 def _check_floats(name: str, t, shape, like):
-    _check(t.is_cuda and t.dtype == torch.float32 and t.is_contiguous(),
-           f"{name} must be a contiguous CUDA float32 tensor")
-    _check(tuple(t.shape) == tuple(shape), f"{name} must have shape {tuple(shape)}")
-    _same_device(like, **{name: t})
+    if not (t.is_cuda and t.dtype == torch.float32 and t.is_contiguous()):
+        raise RuntimeError(f"{name} must be a contiguous CUDA float32 tensor")
+    if t.shape != shape:
+        raise RuntimeError(f"{name} must have shape {tuple(shape)}")
+    _same_device(like, name, t)
 
 
 def _grouped_out(out, A, M: int, N: int, dtype):
     """(result, zero_rest): a new result whose rows outside the groups become
     zeros, or the given one, whose rows there stay."""
     if out is None:
-        return torch.empty((M, N), device=A.device, dtype=dtype), 1
-    _check(out.is_cuda and out.is_contiguous() and tuple(out.shape) == (M, N) and out.dtype == dtype,
-           f"out must be a contiguous CUDA tensor of shape {(M, N)} and type {dtype}")
-    _same_device(A, out=out)
+        return A.new_empty((M, N), dtype=dtype), 1
+    if not (out.is_cuda and out.is_contiguous() and out.shape == (M, N) and out.dtype == dtype):
+        raise RuntimeError(f"out must be a contiguous CUDA tensor of shape {(M, N)} and type {dtype}")
+    _same_device(A, "out", out)
     return out, 0
 
 
@@ -88,8 +96,8 @@ def quantize_rows_int8(x: torch.Tensor):
     with an infinity or a NaN gets a scale that is not finite."""
     _check(x.is_cuda and x.dtype in _TYPES and x.is_contiguous() and x.dim() >= 1,
            "x must be a contiguous CUDA float32, float16 or bfloat16 tensor with at least one axis")
-    codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    codes = torch.empty_like(x, dtype=torch.int8)
+    scales = x.new_empty(x.shape[:-1], dtype=torch.float32)
     _call("tcg_quantize_rows_s8", x, x.data_ptr(), _TYPES[x.dtype], codes.data_ptr(), scales.data_ptr(),
           scales.numel(), x.size(-1))
     return codes, scales
@@ -108,38 +116,38 @@ def gemm_int8_scaled(A: torch.Tensor, BT: torch.Tensor, scale_a: torch.Tensor, s
     _check(A.size(-1) == BT.size(-1), "A cols must equal BT cols (both = K)")
     _check(A.is_contiguous() and BT.is_contiguous(), "A and BT must be contiguous")
     _check(out_dtype in _TYPES, "out_dtype must be float16, bfloat16 or float32")
-    _same_device(A, BT=BT)
+    _same_device(A, "BT", BT)
     lead, M, N, K = A.shape[:-2], A.size(-2), BT.size(-2), A.size(-1)
     _check_floats("scale_a", scale_a, lead + (M,), A)
     _check_floats("scale_b", scale_b, lead + (N,), A)
     if bias is not None:
         _check_floats("bias", bias, lead + (N,), A)
-    C = torch.empty(lead + (M, N), dtype=out_dtype, device=A.device)
+    C = A.new_empty(lead + (M, N), dtype=out_dtype)
     _call("tcg_gemm_s8_scaled", A, A.data_ptr(), BT.data_ptr(), C.data_ptr(), _TYPES[out_dtype], M, N, K,
           A.size(0) if A.dim() == 3 else 1, scale_a.data_ptr(), scale_b.data_ptr(), _ptr(bias))
     return C
 
 
-def _linear_int8(x, BT, offsets, scale_b, bias, out, fn):
+def _linear_int8(x, BT, offsets, scale_b, bias, out):
     groups, N, K = (BT.size(0) if offsets is not None else 1), BT.size(-2), BT.size(-1)
     _check(x.dtype in _TYPES, "x must be float32, float16 or bfloat16")
     _check(BT.dtype == torch.int8, "BT must be int8")
     _check(x.size(-1) == K, "x cols must equal BT cols (both = K)")
     _check(x.is_contiguous() and BT.is_contiguous(), "x and BT must be contiguous")
-    _same_device(x, BT=BT)
+    _same_device(x, "BT", BT)
     _check_floats("scale_b", scale_b, BT.shape[:-1], x)
     if bias is not None:
         _check_floats("bias", bias, BT.shape[:-1], x)
     M = x.numel() // K if K else 0
     _check(K > 0, "K must not be 0")
     if offsets is None:
-        C, rest = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=x.device), 0
+        C, rest = x.new_empty(x.shape[:-1] + (N,)), 0
     else:
         C, rest = _grouped_out(out, x, M, N, x.dtype)
     if C.numel() == 0:
         return C
     need = ((M * K + 255) & ~255) + ((4 * M + 255) & ~255)  # tcg_linear_s8_workspace_size
-    ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+    ws = x.new_empty(need, dtype=torch.uint8)
     _call("tcg_linear_s8_grouped", x, x.data_ptr(), _TYPES[x.dtype], BT.data_ptr(), C.data_ptr(), _TYPES[x.dtype],
           _ptr(offsets), groups, M, N, K, scale_b.data_ptr(), _ptr(bias), rest, ws.data_ptr(), need)
     return C
@@ -152,7 +160,7 @@ def linear_int8(x: torch.Tensor, BT: torch.Tensor, scale_b: torch.Tensor,
     activations to activations (gemm_int8_scaled between)."""
     _check(x.is_cuda and BT.is_cuda, "x and BT must be CUDA tensors")
     _check(x.dim() >= 1 and BT.dim() == 2, "BT must be 2-D")
-    return _linear_int8(x, BT, None, scale_b, bias, None, "linear_int8")
+    return _linear_int8(x, BT, None, scale_b, bias, None)
 
 
 def linear_int8_grouped(x: torch.Tensor, BT: torch.Tensor, offsets: torch.Tensor, scale_b: torch.Tensor,
@@ -162,7 +170,7 @@ def linear_int8_grouped(x: torch.Tensor, BT: torch.Tensor, offsets: torch.Tensor
     _check(x.is_cuda and BT.is_cuda, "x and BT must be CUDA tensors")
     _check(x.dim() == 2 and BT.dim() == 3, "x must be 2-D and BT 3-D")
     _check_offsets(offsets, BT.size(0), x)
-    return _linear_int8(x, BT, offsets, scale_b, bias, out, "linear_int8_grouped")
+    return _linear_int8(x, BT, offsets, scale_b, bias, out)
 
 
 def gemm_int8_grouped(A: torch.Tensor, BT: torch.Tensor, offsets: torch.Tensor, scale_a: torch.Tensor,
@@ -176,7 +184,7 @@ def gemm_int8_grouped(A: torch.Tensor, BT: torch.Tensor, offsets: torch.Tensor, 
     _check(A.size(-1) == BT.size(-1), "A cols must equal BT cols (both = K)")
     _check(A.is_contiguous() and BT.is_contiguous(), "A and BT must be contiguous")
     _check(out_dtype in _TYPES, "out_dtype must be float16, bfloat16 or float32")
-    _same_device(A, BT=BT)
+    _same_device(A, "BT", BT)
     E, N, K = BT.shape
     M = A.size(0)
     _check_offsets(offsets, E, A)
@@ -216,7 +224,7 @@ def gemm_grouped(A: torch.Tensor, B: torch.Tensor, offsets: torch.Tensor, b_layo
     _check(A.is_contiguous() and B.is_contiguous(), "A and B must be contiguous")
     out_dtype = A.dtype if out_dtype is None else out_dtype
     _check(out_dtype in _TYPES, "out_dtype must be float16, bfloat16 or float32")
-    _same_device(A, B=B)
+    _same_device(A, "B", B)
     _check_offsets(offsets, B.size(0), A)
     C, rest = _grouped_out(out, A, A.size(0), N, out_dtype)
     return _product(A, B, offsets, b_layout, C, rest)
@@ -226,7 +234,7 @@ def _wgrad(dC, A, scale_a, offsets, groups, out_dtype):
     """dB[groups,N,K] through tcg_gemm_16_grouped_wgrad (arguments checked)."""
     N, K = dC.size(-1), A.size(-1)
     M = dC.numel() // N if N else 0
-    dB = torch.empty((groups, N, K), dtype=out_dtype, device=dC.device)
+    dB = dC.new_empty((groups, N, K), dtype=out_dtype)
     _call("tcg_gemm_16_grouped_wgrad", dC, dC.data_ptr(), A.data_ptr(), _ptr(scale_a), _TYPES[dC.dtype],
           dB.data_ptr(), _TYPES[out_dtype], _ptr(offsets), groups, M, N, K)
     return dB
@@ -247,7 +255,7 @@ def gemm_grouped_wgrad(dC: torch.Tensor, A: torch.Tensor, offsets: torch.Tensor,
     _check(dC.is_contiguous() and A.is_contiguous(), "dC and A must be contiguous")
     out_dtype = dC.dtype if out_dtype is None else out_dtype
     _check(out_dtype in _TYPES, "out_dtype must be float16, bfloat16 or float32")
-    _same_device(dC, A=A)
+    _same_device(dC, "A", A)
     groups = offsets.numel() - 1
     _check_offsets(offsets, groups, dC)
     if scale_a is not None:
@@ -257,38 +265,56 @@ def gemm_grouped_wgrad(dC: torch.Tensor, A: torch.Tensor, offsets: torch.Tensor,
 
 # ------------------------------------------------------------------ layers --
 
+def _forward(x, W, offsets):
+    return _product(x, W, offsets, "nk", x.new_empty(x.shape[:-1] + (W.size(-2),)), 1)
+
+
+def _backward(ctx, dy):
+    x, scales, W, offsets = ctx.saved_tensors
+    dy = dy.contiguous()
+    dx = dW = None
+    if W is not None:
+        dx = _product(dy, W, offsets, "kn", dy.new_empty(dy.shape[:-1] + (W.size(-1),)), 1)
+    if x is not None:
+        shape = ctx.weight_shape
+        dW = _wgrad(dy, x, scales, offsets, shape[0] if len(shape) == 3 else 1, dy.dtype)
+        if len(shape) == 2:
+            dW = dW.view(shape)
+    return dx, dW, None, None
+
+
+_backward_once = torch.autograd.function.once_differentiable(_backward)
+
+
 class _Linear(torch.autograd.Function):
     """y = x W^T per group.  Backward: dx = dy W (the same product with W's
-    other layout), dW = dy^T x from x or from its int8 codes and scales."""
+    other layout), dW = dy^T x from x or from its int8 codes and scales.  What
+    one input's gradient alone needs is kept only where that is asked for."""
 
     @staticmethod
-    def forward(ctx, x, W, offsets, save):
-        y = torch.empty(x.shape[:-1] + (W.size(-2),), dtype=x.dtype, device=x.device)
-        _product(x, W, offsets, "nk", y, 1)
-        codes = scales = None
-        if ctx.needs_input_grad[1]:
-            if save == "int8":
-                codes, scales = quantize_rows_int8(x)
-                x = None
-        else:
+    def forward(ctx, x, W, offsets, eight):
+        y = _forward(x, W, offsets)
+        need_x, need_W = ctx.needs_input_grad[:2]
+        scales = None
+        if not need_W:
             x = None
-        ctx.save_for_backward(x, codes, scales, W if ctx.needs_input_grad[0] else None, offsets)
+        elif eight:
+            x, scales = quantize_rows_int8(x)
         ctx.weight_shape = W.shape
+        ctx.save_for_backward(x, scales, W if need_x else None, offsets)
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, codes, scales, W, offsets = ctx.saved_tensors
-        dy = dy.contiguous()
-        dx = dW = None
-        if W is not None:
-            dx = torch.empty(dy.shape[:-1] + (W.size(-1),), dtype=dy.dtype, device=dy.device)
-            _product(dy, W, offsets, "kn", dx, 1)
-        if ctx.needs_input_grad[1]:
-            groups = ctx.weight_shape[0] if len(ctx.weight_shape) == 3 else 1
-            dW = _wgrad(dy, codes if x is None else x, scales, offsets, groups, dy.dtype).view(ctx.weight_shape)
-        return dx, dW, None, None
+        # (the wrapper that refuses a second differentiation costs microseconds
+        # and matters only where this one is recorded)
+        return _backward_once(ctx, dy) if torch.is_grad_enabled() else _backward(ctx, dy)
+
+
+def _apply(x, W, offsets, save):
+    if torch.is_grad_enabled() and (x.requires_grad or W.requires_grad):
+        return _Linear.apply(x, W, offsets, save == "int8")
+    return _forward(x, W, offsets)
 
 
 def _check_linear(x, W, save):
@@ -300,7 +326,7 @@ def _check_linear(x, W, save):
     _check(W.size(-1) % (16 if save == "int8" else 8) == 0, "K must be a multiple of 8 (16 with save='int8')")
     _check(W.size(-2) % 8 == 0, "N must be a multiple of 8")
     _check(W.numel() > 0, "W must not be empty")
-    _same_device(x, W=W)
+    _same_device(x, "W", W)
 
 
 def linear(x: torch.Tensor, W: torch.Tensor, save: str = "input") -> torch.Tensor:
@@ -310,7 +336,7 @@ def linear(x: torch.Tensor, W: torch.Tensor, save: str = "input") -> torch.Tenso
     gradient are unchanged, W's gradient is that of the codes."""
     _check(x.dim() >= 1 and W.dim() == 2, "W must be 2-D")
     _check_linear(x, W, save)
-    return _Linear.apply(x, W, None, save)
+    return _apply(x, W, None, save)
 
 
 def linear_grouped(x: torch.Tensor, W: torch.Tensor, offsets: torch.Tensor, save: str = "input") -> torch.Tensor:
@@ -319,7 +345,7 @@ def linear_grouped(x: torch.Tensor, W: torch.Tensor, offsets: torch.Tensor, save
     _check(x.dim() == 2 and W.dim() == 3, "x must be 2-D and W 3-D")
     _check_linear(x, W, save)
     _check_offsets(offsets, W.size(0), x)
-    return _Linear.apply(x, W, offsets, save)
+    return _apply(x, W, offsets, save)
 
 
 def set_rows_tile(rows: int, split: int = 0) -> None:
