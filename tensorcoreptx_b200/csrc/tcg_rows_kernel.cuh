@@ -399,16 +399,25 @@ __device__ __forceinline__ void conv_scales(const RowsParams& p, int r0, int ren
     }
 }
 
+// Which half of its 16 codes a thread takes first: the other one in threads
+// 4..7 of a row and in odd rows, so that neither reads nor writes (16 bytes of
+// eight threads, two rows of 8-byte reads) meet in a bank.
+__device__ __forceinline__ int conv_first(int ct) { return ((ct >> 2) ^ (ct >> 3)) & 1; }
+
 // pass u of block b is 16 codes of row u * kConvRows + ct / 8
 template <class C>
 __device__ __forceinline__ void conv_codes(const uint8_t* raw, int ct, ConvRegs<C>& g)
 {
+    const int first = conv_first(ct) * 8;
 #pragma unroll
     for (int b = 0; b < C::kSub; ++b)
 #pragma unroll
-        for (int u = 0; u < g.kPerBlock; ++u)
-            g.v[b * g.kPerBlock + u] = *reinterpret_cast<const uint4*>(
-                raw + (u * kConvRows + (ct >> 3)) * C::kTileP + b * 128 + (ct & 7) * 16);
+        for (int u = 0; u < g.kPerBlock; ++u) {
+            const uint8_t* at = raw + (u * kConvRows + (ct >> 3)) * C::kTileP + b * 128 + (ct & 7) * 16;
+            const uint2 x = *reinterpret_cast<const uint2*>(at + first);
+            const uint2 y = *reinterpret_cast<const uint2*>(at + (first ^ 8));
+            g.v[b * g.kPerBlock + u] = make_uint4(x.x, x.y, y.x, y.y);
+        }
 }
 
 __device__ __forceinline__ float code_float(uint32_t w, int i)
@@ -420,7 +429,7 @@ __device__ __forceinline__ float code_float(uint32_t w, int i)
 template <class C, bool kBf16>
 __device__ __forceinline__ void conv_write(uint8_t* p_area, int ct, const ConvRegs<C>& g)
 {
-    const int c = ct & 7;
+    const int c = ct & 7, first = conv_first(ct);
 #pragma unroll
     for (int b = 0; b < C::kSub; ++b)
 #pragma unroll
@@ -437,8 +446,8 @@ __device__ __forceinline__ void conv_write(uint8_t* p_area, int ct, const ConvRe
                 ow[2 * i + 1] = pack16<kBf16>(code_float(in[i], 2) * s, code_float(in[i], 3) * s);
             }
             uint8_t* row = p_area + b * C::kSubBytes + (c >> 2) * C::kAtomBytes + r * 128;
-            *reinterpret_cast<uint4*>(row + (((2 * (c & 3)) ^ (r & 7)) << 4)) = o[0];
-            *reinterpret_cast<uint4*>(row + (((2 * (c & 3) + 1) ^ (r & 7)) << 4)) = o[1];
+            *reinterpret_cast<uint4*>(row + (((2 * (c & 3) + first) ^ (r & 7)) << 4)) = o[0];
+            *reinterpret_cast<uint4*>(row + (((2 * (c & 3) + (first ^ 1)) ^ (r & 7)) << 4)) = o[1];
         }
 }
 
@@ -722,13 +731,12 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
             const int blocks = blocks_of(w);
             // columns of the MMA: the tile's rows rounded up to what the instruction takes
             const int n = w.cnt <= 16 ? 16 : (w.cnt + 31) & ~31;
-            const uint32_t idesc = p.idesc | (static_cast<uint32_t>(n >> 3) << 17);
+            const uint32_t idesc = __shfl_sync(0xffffffffu, p.idesc | (static_cast<uint32_t>(n >> 3) << 17), 0);
             // stage st, k-block kb: operands in shared memory
             const auto ready = [&](int st, uint32_t ph) {
-                return wait_bounded_warp(smem_u32(&full[st]), ph, abort_flag, p.timeout_ns,
-                                         (blockIdx.x << 8) | 0x30u | st) &&
-                       (!C::kConv || wait_bounded_warp(smem_u32(&conv[st]), ph, abort_flag, p.timeout_ns,
-                                                       (blockIdx.x << 8) | 0xB0u | st));
+                // (kConv: the converters waited for the stage's copies before they arrived)
+                return wait_bounded_warp(smem_u32(C::kConv ? &conv[st] : &full[st]), ph, abort_flag, p.timeout_ns,
+                                         (blockIdx.x << 8) | 0x30u | st);
             };
             // The sum ends inside an MMA step of the last k-block: the step's
             // remaining rows belong to the next group and are overwritten with
@@ -751,9 +759,11 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
             // `mask`; a descriptor's low word is an address in 16-byte units
             const auto issue = [&](int st, int kb, int mask) {
                 tc_fence_after();
+                // (broadcasts, so that the compiler knows the operands to be uniform)
+                const uint64_t at = static_cast<uint64_t>(__shfl_sync(0xffffffffu, st, 0)) * (C::kStageBytes / 16);
+                const int ksteps =
+                    __shfl_sync(0xffffffffu, (valid_of(w, kb) + C::kUmmaK - 1) / C::kUmmaK, 0);
                 if (elect_one()) {
-                    const int ksteps = (valid_of(w, kb) + C::kUmmaK - 1) / C::kUmmaK;
-                    const uint64_t at = static_cast<uint64_t>(st) * (C::kStageBytes / 16);
 #pragma unroll
                     for (int k = 0; k < C::kBK / C::kUmmaK; ++k) {
                         if (k >= ksteps) break;
@@ -932,7 +942,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                 return OutBlock{p.out, row + c, p.P, w.p0 + h * 128, min(32, w.cnt - c),
                                 min(128, p.P - w.p0 - h * 128), p.aligned_out != 0};
             };
-            if (C::kHold && p.out_type != kOutF32) {
+            if (C::kHold && p.out_type != kOutF32 && p.aligned_out) {
                 // Both blocks into registers (128 words a thread) before any
                 // store: the accumulators are free for the next tile after
                 // about 3000 cycles instead of the 11000 that the stores of
@@ -963,12 +973,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                     for (int i = 0; i < 4; ++i) {
                         const int c = 32 * group + 64 * i;
                         const OutBlock o = block_of(h, c);
-                        if (c < w.cnt && o.features > 0) {
-                            if (o.aligned)
-                                store_block16(held[h][i], o, stage_out, quarter, lane, 2 + group);
-                            else
-                                store_rows16(held[h][i], o, quarter, lane);
-                        }
+                        if (c < w.cnt && o.features > 0) store_block16(held[h][i], o, stage_out, quarter, lane, 2 + group);
                     }
             } else {
                 for (int h = 0; h < C::kSub; ++h) {
