@@ -135,10 +135,13 @@ tcg_status tcg_quantize_absmax_s4(const float* src, int8_t* dst_packed, int rows
  * every step in IEEE single precision; a row of zeros has scale 0 and codes 0,
  * a row with an infinity or NaN a scale that is not finite.  src and scale
  * need their element's alignment only; rows of whole 16-byte vectors at a
- * 16-byte aligned src take the faster path.  The left operand of the next
- * three. */
+ * 16-byte aligned src take the faster path.
+ * tcg_dequantize_rows_s8 is the way back: dst = code * scale of the row in
+ * single precision, rounded to `type`. */
 tcg_status tcg_quantize_rows_s8(const void* src, tcg_dtype type, int8_t* dst, float* scale, long long rows, int k,
                                 void* stream);
+tcg_status tcg_dequantize_rows_s8(const int8_t* src, const float* scale, void* dst, tcg_dtype type, long long rows,
+                                  int k, void* stream);
 
 /* Products of int8 rows with a scale each and int8 weights with a scale per
  * output channel (B is N x K, "BT"):
@@ -170,17 +173,15 @@ tcg_status tcg_linear_s8(const void* x, tcg_dtype x_type, const int8_t* B, void*
  * of the gradient by C with B in the other layout.
  * tcg_gemm_16_grouped_wgrad: the gradient by B of the TCG_B_NK product:
  *   dB[e][n][k] = sum over the rows m of group e of dC[m][n] * A[m][k]
- * (zeros for an empty group), N % 8 == 0 and K % 8 == 0.  With scale_a, A holds
- * int8 codes with a scale per row (tcg_quantize_rows_s8; K % 16 == 0) and
- * stands for scale_a[m] * A[m][k] rounded to `type`.
+ * (zeros for an empty group), N % 8 == 0 and K % 8 == 0.
  * tcg_gemm_s8_grouped / tcg_linear_s8_grouped: as tcg_gemm_s8_scaled /
  * tcg_linear_s8 with scale_b and bias groups x N. */
 #define TCG_MAX_GROUPS 1024
 tcg_status tcg_gemm_16_grouped(const void* A, const void* B, tcg_dtype type, void* C, tcg_dtype c_type,
                                const int32_t* offsets, int groups, int M, int N, int K, tcg_b_layout b_layout,
                                int zero_rest, void* stream);
-tcg_status tcg_gemm_16_grouped_wgrad(const void* dC, const void* A, const float* scale_a, tcg_dtype type, void* dB,
-                                     tcg_dtype b_type, const int32_t* offsets, int groups, int M, int N, int K,
+tcg_status tcg_gemm_16_grouped_wgrad(const void* dC, const void* A, tcg_dtype type, void* dB, tcg_dtype b_type,
+                                     const int32_t* offsets, int groups, int M, int N, int K,
                                      void* stream);
 tcg_status tcg_gemm_s8_grouped(const int8_t* A, const int8_t* B, void* C, tcg_dtype c_type, const int32_t* offsets,
                                int groups, int M, int N, int K, const float* scale_a, const float* scale_b,

@@ -15,13 +15,13 @@ from .gemm import (check_device_error, gemm_fp8, gemm_int4_dequant, gemm_int8_de
                    quantize_absmax_int8, gemm_fp16, gemm_fp16_nk, gemm_int4, gemm_int8,
                    gemm_int8_kn, int4_workspace_size, last_tile_m, last_tile_n, set_cta_pair,
                    set_tile_n, unpack_int4)
-from .rows import (gemm_grouped, gemm_grouped_wgrad, gemm_int8_grouped, gemm_int8_scaled, linear, linear_grouped,
-                   linear_int8, linear_int8_grouped, quantize_rows_int8, set_rows_tile)
+from .rows import (dequantize_rows_int8, gemm_grouped, gemm_grouped_wgrad, gemm_int8_grouped, gemm_int8_scaled, linear,
+                   linear_grouped, linear_int8, linear_int8_grouped, quantize_rows_int8, set_rows_tile)
 
 __all__ = ["gemm_fp16", "gemm_fp16_nk", "gemm_int8", "gemm_int8_kn", "gemm_int4",
            "int4_workspace_size", "unpack_int4", "check_device_error", "set_tile_n",
            "last_tile_n", "last_tile_m", "set_cta_pair", "gemm_int8_host", "gemm_fp16_host",
            "quantize_absmax_int8", "quantize_absmax_int4", "gemm_int8_dequant", "gemm_int4_dequant",
-           "gemm_fp8", "quantize_rows_int8", "gemm_int8_scaled", "linear_int8", "gemm_grouped",
+           "gemm_fp8", "quantize_rows_int8", "dequantize_rows_int8", "gemm_int8_scaled", "linear_int8", "gemm_grouped",
            "gemm_grouped_wgrad", "gemm_int8_grouped", "linear_int8_grouped", "linear", "linear_grouped",
            "set_rows_tile"]

@@ -42,11 +42,12 @@ SIGNATURES = {
     "tcg_quantize_absmax_s8": (C.c_int, [_p, _p, _sz, _p, _p]),
     "tcg_quantize_absmax_s4": (C.c_int, [_p, _p, _i, _i, _p, _p]),
     "tcg_quantize_rows_s8": (C.c_int, [_p, _i, _p, _p, C.c_longlong, _i, _p]),
+    "tcg_dequantize_rows_s8": (C.c_int, [_p, _p, _p, _i, C.c_longlong, _i, _p]),
     "tcg_gemm_s8_scaled": (C.c_int, [_p, _p, _p, _i, _i, _i, _i, _i, _p, _p, _p, _p]),
     "tcg_linear_s8_workspace_size": (_sz, [_i, _i]),
     "tcg_linear_s8": (C.c_int, [_p, _i, _p, _p, _i, _i, _i, _i, _p, _p, _p, _sz, _p]),
     "tcg_gemm_16_grouped": (C.c_int, [_p, _p, _i, _p, _i, _p, _i, _i, _i, _i, _i, _i, _p]),
-    "tcg_gemm_16_grouped_wgrad": (C.c_int, [_p, _p, _p, _i, _p, _i, _p, _i, _i, _i, _i, _p]),
+    "tcg_gemm_16_grouped_wgrad": (C.c_int, [_p, _p, _i, _p, _i, _p, _i, _i, _i, _i, _p]),
     "tcg_gemm_s8_grouped": (C.c_int, [_p, _p, _p, _i, _p, _i, _i, _i, _i, _p, _p, _p, _i, _p]),
     "tcg_linear_s8_grouped": (C.c_int, [_p, _i, _p, _p, _i, _p, _i, _i, _i, _i, _p, _p, _i, _p, _sz, _p]),
     "tcg_gemm_s4_static": (C.c_int, [_p, _p, _p, _i, _i, _i, _i, _p]),

@@ -246,6 +246,42 @@ __global__ void __launch_bounds__(kRowThreads)
     }
 }
 
+// The way back: code * scale[row] in fp32, rounded once to T (at most half a
+// step of T, against the half code step, 2^-8 of the row's largest value, that
+// the codes are off by).  kCodes codes a thread and step, whole rows of them
+// (kCodes = 16: one 16-byte load) or one by one.  HBM bound: 1 byte read and 2
+// (4) written a value.
+template <class T>
+__device__ __forceinline__ T row_result(float f) { return T(f); }
+
+template <class T, int kCodes>
+__global__ void __launch_bounds__(kRowThreads)
+    dequantize_rows_kernel(const int8_t* __restrict__ q, const float* __restrict__ scale, T* __restrict__ out,
+                           long long rows, int k)
+{
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const int per_row = k / kCodes;
+    const long long total = rows * per_row;
+    const long long stride = static_cast<long long>(gridDim.x) * kRowThreads;
+    for (long long i = static_cast<long long>(blockIdx.x) * kRowThreads + threadIdx.x; i < total; i += stride) {
+        const float s = scale[total <= 0x7fffffffLL ? static_cast<int>(i) / per_row : i / per_row];
+        if constexpr (kCodes == 16) {
+            const uint4 v = reinterpret_cast<const uint4*>(q)[i];
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            alignas(16) T o[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                o[j] = row_result<T>(static_cast<float>(static_cast<int8_t>(w[j / 4] >> (8 * (j % 4)))) * s);
+            uint4* to = reinterpret_cast<uint4*>(out) + i * sizeof(T);
+#pragma unroll
+            for (int j = 0; j < static_cast<int>(sizeof(T)); ++j) to[j] = reinterpret_cast<const uint4*>(o)[j];
+        } else {
+            out[i] = row_result<T>(static_cast<float>(q[i]) * s);
+        }
+    }
+}
+
 // *scale = absmax / qmax, written over the absmax slot once every quantise
 // block has read it (stream order).
 __global__ void publish_scale_kernel(float* scale_and_absmax, float qmax)

@@ -25,14 +25,14 @@ std::atomic<int> g_rows_split{0};
 
 // One product, checked and ready to launch.
 struct RowsCall {
-    const void* pside;      // weights; weight form: the rows' other side (16-bit values or int8 codes)
+    const void* pside;      // weights; weight form: the rows' other side
     const void* qside;      // rows; weight form: the gradient by the product's result
     void* out;
     int out_type;
     bool bf16;
     const int32_t* offsets;
     int groups, rows, P, Q, R;
-    const float *scale_q, *scale_p, *bias_p, *scale_r;
+    const float *scale_q, *scale_p, *bias_p;
     int zero_rest;
     int early;
 };
@@ -112,8 +112,7 @@ tcg_status launch(const RowsCall& c, int split, int dev, int sms, cudaStream_t s
         smem_set[dev].store(true, std::memory_order_release);
     }
 
-    const CUtensorMapDataType t16 = CU_TENSOR_MAP_DATA_TYPE_UINT16, t8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
-    const CUtensorMapDataType dt = C::kElem == 2 ? t16 : t8;
+    const CUtensorMapDataType dt = C::kElem == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
     const uint64_t es = C::kElem, P = c.P, Q = c.Q, R = c.R, M = c.rows, G = c.groups;
     const CUtensorMapSwizzle swz = CU_TENSOR_MAP_SWIZZLE_128B;
     // An MN-major operand of whole 64-element atoms is seen as {64, rows, atoms,
@@ -132,10 +131,7 @@ tcg_status launch(const RowsCall& c, int split, int dev, int sms, cudaStream_t s
     };
     CUtensorMap mp, mq, mqb;  // mqb: rows in boxes of kQBox, for tiles that are not full
     tcg_status s;
-    if (C::kConv)
-        s = host::encode_4d(&mp, t8, c.pside, {{P, M, 1, 1}, {P, M * P, M * P}, {C::kTileP, bk, 1}},
-                            CU_TENSOR_MAP_SWIZZLE_NONE);
-    else if (C::kWeight)
+    if (C::kWeight)
         s = host::encode_4d(&mp, dt, c.pside, atoms(P, M, 1, p_whole, 2 * C::kSub), swz);
     else if (C::kPMn)
         s = host::encode_4d(&mp, dt, c.pside, atoms(P, R, G, p_whole, 2 * C::kSub), swz);
@@ -156,7 +152,6 @@ tcg_status launch(const RowsCall& c, int split, int dev, int sms, cudaStream_t s
     p.scale_q = c.scale_q;
     p.scale_p = c.scale_p;
     p.bias_p = c.bias_p;
-    p.scale_r = c.scale_r;
     p.timeout_ns = host::wait_timeout_ns();
     p.groups = c.groups;
     p.rows = c.rows;
@@ -170,7 +165,6 @@ tcg_status launch(const RowsCall& c, int split, int dev, int sms, cudaStream_t s
     const int out_bytes = c.out_type == kOutF32 ? 4 : 2;
     p.aligned_out = (static_cast<long long>(c.P) * out_bytes) % 16 == 0 && (reinterpret_cast<uintptr_t>(c.out) & 15u) == 0;
     p.out_type = c.out_type;
-    p.bf16 = c.bf16;
     while ((1 << p.split_log2) < split) ++p.split_log2;
     p.early = c.early;
     p.p_whole = p_whole;
@@ -241,23 +235,22 @@ tcg_status run_rows(const RowsCall& c, cudaStream_t st)
     if (s != TCG_SUCCESS) return s;
     const RowsPlan plan = choose_plan(c, false, kKind == kKindF16 ? 64 : 128, sms);
     switch (plan.bq) {
-    case 16: return launch<RowsTraits<kKind, kPMn, false, false, 1, 16>>(c, plan.split, dev, sms, st);
-    case 32: return launch<RowsTraits<kKind, kPMn, false, false, 1, 32>>(c, plan.split, dev, sms, st);
-    case 64: return launch<RowsTraits<kKind, kPMn, false, false, 1, 64>>(c, plan.split, dev, sms, st);
-    case 128: return launch<RowsTraits<kKind, kPMn, false, false, 1, 128>>(c, plan.split, dev, sms, st);
-    default: return launch<RowsTraits<kKind, kPMn, false, false, 2, 256>>(c, 1, dev, sms, st);
+    case 16: return launch<RowsTraits<kKind, kPMn, false, 1, 16>>(c, plan.split, dev, sms, st);
+    case 32: return launch<RowsTraits<kKind, kPMn, false, 1, 32>>(c, plan.split, dev, sms, st);
+    case 64: return launch<RowsTraits<kKind, kPMn, false, 1, 64>>(c, plan.split, dev, sms, st);
+    case 128: return launch<RowsTraits<kKind, kPMn, false, 1, 128>>(c, plan.split, dev, sms, st);
+    default: return launch<RowsTraits<kKind, kPMn, false, 2, 256>>(c, 1, dev, sms, st);
     }
 }
 
-template <bool kConv>
 tcg_status run_weight(const RowsCall& c, cudaStream_t st)
 {
     int dev, sms;
     const tcg_status s = host::device(&dev, &sms);
     if (s != TCG_SUCCESS) return s;
     const RowsPlan plan = choose_plan(c, true, 64, sms);
-    if (plan.bq == 256) return launch<RowsTraits<kKindF16, true, true, kConv, 2, 256>>(c, 1, dev, sms, st);
-    return launch<RowsTraits<kKindF16, true, true, kConv, 1, 128>>(c, plan.split, dev, sms, st);
+    if (plan.bq == 256) return launch<RowsTraits<kKindF16, true, true, 2, 256>>(c, 1, dev, sms, st);
+    return launch<RowsTraits<kKindF16, true, true, 1, 128>>(c, plan.split, dev, sms, st);
 }
 
 bool is_type(tcg_dtype t) { return t == TCG_F32 || t == TCG_F16 || t == TCG_BF16; }
@@ -416,8 +409,8 @@ tcg_status tcg_gemm_16_grouped(const void* A, const void* B, tcg_dtype type, voi
     return b_layout == TCG_B_NK ? run_rows<kKindF16, false>(c, st) : run_rows<kKindF16, true>(c, st);
 }
 
-tcg_status tcg_gemm_16_grouped_wgrad(const void* dC, const void* A, const float* scale_a, tcg_dtype type, void* dB,
-                                     tcg_dtype b_type, const int32_t* offsets, int groups, int M, int N, int K,
+tcg_status tcg_gemm_16_grouped_wgrad(const void* dC, const void* A, tcg_dtype type, void* dB, tcg_dtype b_type,
+                                     const int32_t* offsets, int groups, int M, int N, int K,
                                      void* stream)
 {
     if ((type != TCG_F16 && type != TCG_BF16) || !is_type(b_type)) return TCG_ERR_ARG;
@@ -427,8 +420,8 @@ tcg_status tcg_gemm_16_grouped_wgrad(const void* dC, const void* A, const float*
     if (s != TCG_SUCCESS || done) return s;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (!dB) return TCG_ERR_ARG;
-    if (N % 8 != 0 || K % (scale_a ? 16 : 8) != 0) return TCG_ERR_SHAPE;
-    if (misaligned(dB, size_of(b_type)) || misaligned(scale_a, 4)) return TCG_ERR_ALIGN;
+    if (N % 8 != 0 || K % 8 != 0) return TCG_ERR_SHAPE;
+    if (misaligned(dB, size_of(b_type))) return TCG_ERR_ALIGN;
     if (M == 0) {  // no rows at all: every gradient is zero
         const cudaError_t e = cudaMemsetAsync(dB, 0, static_cast<size_t>(weights) * K * size_of(b_type), st);
         return e == cudaSuccess ? TCG_SUCCESS : host::fail(e);
@@ -447,8 +440,7 @@ tcg_status tcg_gemm_16_grouped_wgrad(const void* dC, const void* A, const float*
     c.rows = M;
     c.P = K;
     c.Q = N;
-    c.scale_r = scale_a;
-    return scale_a ? run_weight<true>(c, st) : run_weight<false>(c, st);
+    return run_weight(c, st);
 }
 
 void tcg_set_rows_tile(int rows, int split)

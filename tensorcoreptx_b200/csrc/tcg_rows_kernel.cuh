@@ -28,9 +28,8 @@
 //   kSub = 2: 256 x 256, persistent CTAs, two M = 128 accumulators that fill
 //     the tensor memory.  For many rows, where the tensor cores bound it.
 //
-// Warps: 0 TMA producer (one thread), 1 MMA issuer, 2..9 epilogue (two per
-// tensor-memory lane quarter), and with kConv eight converter warps (see
-// conv_write).  Every wait on an mbarrier is bounded (tcg_wait.cuh).
+// Warps: 0 TMA producer, 1 MMA issuer, 2..9 epilogue (two per
+// tensor-memory lane quarter).  Every wait on an mbarrier is bounded (tcg_wait.cuh).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -51,7 +50,6 @@ struct RowsParams {
     const float* scale_q;     // int8: one per row
     const float* scale_p;     // int8: one per group and feature
     const float* bias_p;      // int8: one per group and feature, or null
-    const float* scale_r;     // kConv: one per row (the rows are the reduction)
     unsigned long long timeout_ns;
     int groups, rows, rows_per_group;
     int P, Q, R;              // features out; weight form: the other features; rows form: length of the sum
@@ -61,7 +59,6 @@ struct RowsParams {
     int zero_rest;            // rows form: write zeros into rows outside every group
     int aligned_out;          // output rows are whole 16-byte vectors, 16-byte aligned
     int out_type;
-    int bf16;                 // 16-bit operands are bf16 (kConv: type of the widened codes)
     int split_log2;           // kSub = 1: 1, 2, 4 or 8 CTAs per tile
     int stages;               // ring depth
     int p_whole, q_whole;     // MN-major operands of whole 64-element atoms: one copy a tile and stage
@@ -69,46 +66,40 @@ struct RowsParams {
     uint32_t idesc;           // instruction descriptor without N
 };
 
-template <int kKind_, bool kPMn_, bool kQMn_, bool kConv_, int kSub_, int kBQ_>
+template <int kKind_, bool kPMn_, bool kQMn_, int kSub_, int kBQ_>
 struct RowsTraits {
     static constexpr int kKind = kKind_;
-    static constexpr bool kPMn = kPMn_, kQMn = kQMn_, kConv = kConv_;
+    static constexpr bool kPMn = kPMn_, kQMn = kQMn_;
     static constexpr int kSub = kSub_, kBQ = kBQ_;
     static constexpr bool kWeight = kQMn;               // weight form: the sum runs over a group's rows
     static constexpr int kElem = kKind == kKindF16 ? 2 : 1;
-    // length of the sum per ring stage; kConv: a quarter of a row of codes, so that
-    // stages are small and many enough to hide the conversion
-    static constexpr int kBK = kConv ? 32 : 128 / kElem;
+    static constexpr int kBK = 128 / kElem;             // length of the sum per ring stage
     static constexpr int kUmmaK = 32 / kElem;
     static constexpr int kTileP = 128 * kSub;
     static constexpr int kSubBytes = 128 * kBK * kElem; // one 128-feature block of a stage
     static constexpr int kPBytes = kSub * kSubBytes;
     static constexpr int kQBytes = kBQ * kBK * kElem;
-    static constexpr int kRawBytes = 128 * kBK;         // kConv: int8 codes of one 128-feature block
-    static constexpr int kStageBytes = kPBytes + kQBytes + (kConv ? kSub * kRawBytes : 0);
+    static constexpr int kStageBytes = kPBytes + kQBytes;
     static constexpr int kAtomBytes = 128 * kBK;        // MN-major: 64 elements of kBK rows
     static constexpr int kQBox = kBQ < 64 ? kBQ : 64;   // rows (weight form: columns) per box of the q operand
     static constexpr int kQBoxBytes = kQBox * kBK * kElem;
-    static constexpr int kConvWarps = kConv ? 8 : 0;    // two groups of four, taking stages in turn
     static constexpr int kEpiWarps = 8;                 // two per quarter of the tensor memory's lanes
-    static constexpr int kFirstConv = 2 + kEpiWarps;
-    static constexpr int kThreads = 32 * (kFirstConv + kConvWarps);
+    static constexpr int kThreads = 32 * (2 + kEpiWarps);
     // 16-bit results of a whole tile fit the epilogue's registers
-    static constexpr bool kHold = kSub == 2 && !kConv;
-    static constexpr int kPerSm = kSub == 1 && !kConv ? 2 : 1;  // CTAs per SM that registers are kept for
+    static constexpr bool kHold = kSub == 2;
+    static constexpr int kPerSm = kSub == 1 ? 2 : 1;  // CTAs per SM that registers are kept for
     static constexpr int kTmemCols = kSub * kBQ < 32 ? 32 : kSub * kBQ;
     static constexpr int kRedBytes = kBQ * 512;         // split: 128 x kBQ partial sums
     static constexpr int kMaxStages = 12;
-    static constexpr int kBarBytes = 384;
+    static constexpr int kBarBytes = 256;
     static constexpr int kScaleBytes = 1024;            // scales of the rows being written out
     // two blocks of 32 x 128 results on their way out; one tile a CTA: in the ring, which is idle by then
     static constexpr int kOutBytes = 8192;
     static constexpr int kOutArea = kSub == 2 ? 2 * kOutBytes : 0;
-    static_assert(!kConv || (kPMn && kQMn && kKind == kKindF16), "converted operand: weight form only");
     static_assert(!kQMn || kKind == kKindF16, "weight form: 16-bit operands");
     static_assert(!kPMn || kKind == kKindF16, "MN-major features: 16-bit operands");
     static_assert(!kQMn || kBQ % 64 == 0, "whole 64-column atoms");
-    static_assert(8 * (3 * kMaxStages + 5) + 16 <= kBarBytes, "barrier area");
+    static_assert(8 * (2 * kMaxStages + 5) + 16 <= kBarBytes, "barrier area");
     static_assert((kTmemCols & (kTmemCols - 1)) == 0 && kTmemCols <= 512, "TMEM allocation");
     // dynamic shared memory of a launch with a table of `groups` groups
     static constexpr int smem_bytes(int stages, int split, int groups)
@@ -220,6 +211,21 @@ __device__ __forceinline__ RowsItem rows_tile(const RowsParams& p, int pt, int t
     }
     w.cnt = min(C::kBQ, w.rend - w.row0);
     w.nkb = w.zero ? 0 : (p.R + C::kBK - 1) / C::kBK;
+    return w;
+}
+
+// The same tile with every field broadcast, so that the compiler knows what
+// the producer and the MMA issuer compute from it to be uniform.
+__device__ __forceinline__ RowsItem uniform(RowsItem w)
+{
+    const unsigned all = 0xffffffffu;
+    w.e = __shfl_sync(all, w.e, 0);
+    w.row0 = __shfl_sync(all, w.row0, 0);
+    w.cnt = __shfl_sync(all, w.cnt, 0);
+    w.p0 = __shfl_sync(all, w.p0, 0);
+    w.q0 = __shfl_sync(all, w.q0, 0);
+    w.nkb = __shfl_sync(all, w.nkb, 0);
+    w.rend = __shfl_sync(all, w.rend, 0);
     return w;
 }
 
@@ -365,92 +371,6 @@ __device__ __forceinline__ void store_block32(const float (&x)[32], const OutBlo
     }
 }
 
-// kConv: one ring stage of int8 codes (kBK rows of the tile's features) into 16-bit values code * scale[row] in the MN-major
-// 128-byte-swizzled layout the MMA reads: per block two atoms of 64 features,
-// an atom's row r at r * 128 with its 16-byte chunk c at c ^ (r & 7).  The
-// product of code and scale is rounded to 16 bits: at most half a step of
-// the operand type, against half a code step (2^-8 of the row's largest value)
-// that the codes themselves are off by.
-// The codes have an area of their own in the stage, so that no thread waits for
-// another before it writes (in place, with a barrier between reading and
-// writing, a stage took 300 cycles longer).  Eight consecutive threads hold one
-// row.  Rows past the end of the group have scale 0 and become zeros.  The
-// integer pipe bounds this: per four codes one exclusive-or, four byte
-// permutes and two packs at two cycles a warp each.
-constexpr int kConvThreads = 128;
-constexpr int kConvRows = kConvThreads / 8;  // rows of one block per pass
-
-template <class C>
-struct ConvRegs {
-    static constexpr int kPerBlock = C::kBK / kConvRows;
-    uint4 v[kPerBlock * C::kSub];
-    float s[kPerBlock];
-};
-
-// scales of one thread's rows of the k-block that starts at row r0 (rend: end of the group)
-template <class C>
-__device__ __forceinline__ void conv_scales(const RowsParams& p, int r0, int rend, int ct,
-                                            float (&s)[ConvRegs<C>::kPerBlock])
-{
-#pragma unroll
-    for (int u = 0; u < ConvRegs<C>::kPerBlock; ++u) {
-        const int r = r0 + u * kConvRows + (ct >> 3);
-        s[u] = r < rend ? p.scale_r[r] : 0.f;
-    }
-}
-
-// Which half of its 16 codes a thread takes first: the other one in threads
-// 4..7 of a row and in odd rows, so that neither reads nor writes (16 bytes of
-// eight threads, two rows of 8-byte reads) meet in a bank.
-__device__ __forceinline__ int conv_first(int ct) { return ((ct >> 2) ^ (ct >> 3)) & 1; }
-
-// pass u of block b is 16 codes of row u * kConvRows + ct / 8
-template <class C>
-__device__ __forceinline__ void conv_codes(const uint8_t* raw, int ct, ConvRegs<C>& g)
-{
-    const int first = conv_first(ct) * 8;
-#pragma unroll
-    for (int b = 0; b < C::kSub; ++b)
-#pragma unroll
-        for (int u = 0; u < g.kPerBlock; ++u) {
-            const uint8_t* at = raw + (u * kConvRows + (ct >> 3)) * C::kTileP + b * 128 + (ct & 7) * 16;
-            const uint2 x = *reinterpret_cast<const uint2*>(at + first);
-            const uint2 y = *reinterpret_cast<const uint2*>(at + (first ^ 8));
-            g.v[b * g.kPerBlock + u] = make_uint4(x.x, x.y, y.x, y.y);
-        }
-}
-
-__device__ __forceinline__ float code_float(uint32_t w, int i)
-{
-    // byte i of w (biased by 128) in the low mantissa bits of 2^23, minus 2^23 + 128: exact
-    return __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7650 | i)) - 8388736.0f;
-}
-
-template <class C, bool kBf16>
-__device__ __forceinline__ void conv_write(uint8_t* p_area, int ct, const ConvRegs<C>& g)
-{
-    const int c = ct & 7, first = conv_first(ct);
-#pragma unroll
-    for (int b = 0; b < C::kSub; ++b)
-#pragma unroll
-        for (int u = 0; u < g.kPerBlock; ++u) {
-            const int r = u * kConvRows + (ct >> 3);
-            const uint4 v = g.v[b * g.kPerBlock + u];
-            const float s = g.s[u];
-            uint4 o[2];
-            uint32_t* ow = reinterpret_cast<uint32_t*>(o);
-            const uint32_t in[4] = {v.x ^ 0x80808080u, v.y ^ 0x80808080u, v.z ^ 0x80808080u, v.w ^ 0x80808080u};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                ow[2 * i] = pack16<kBf16>(code_float(in[i], 0) * s, code_float(in[i], 1) * s);
-                ow[2 * i + 1] = pack16<kBf16>(code_float(in[i], 2) * s, code_float(in[i], 3) * s);
-            }
-            uint8_t* row = p_area + b * C::kSubBytes + (c >> 2) * C::kAtomBytes + r * 128;
-            *reinterpret_cast<uint4*>(row + (((2 * (c & 3) + first) ^ (r & 7)) << 4)) = o[0];
-            *reinterpret_cast<uint4*>(row + (((2 * (c & 3) + (first ^ 1)) ^ (r & 7)) << 4)) = o[1];
-        }
-}
-
 // Split sums.  Columns c .. c + n - 1 of this CTA's part (one lane = feature
 // f) to the CTAs that finish them: CTA d finishes columns d * kBQ / S onwards.
 // There the parts lie as [source rank][group of V columns][feature][V], V = 4
@@ -543,8 +463,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
     float* scales = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(red) + (S > 1 ? C::kRedBytes : 0));
     uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(scales) + C::kScaleBytes);
     uint64_t* empty = full + C::kMaxStages;
-    uint64_t* conv = empty + C::kMaxStages;  // kConv: stage widened (one arrival per converter warp)
-    uint64_t* tfull = conv + C::kMaxStages;  // accumulator block h complete
+    uint64_t* tfull = empty + C::kMaxStages;  // accumulator block h complete
     uint64_t* tempty = tfull + 2;            // accumulator block h read
     uint64_t* drain = tempty + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
@@ -552,16 +471,15 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
     int* bound = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(full) + C::kBarBytes);
     int* cum = bound + p.groups + 3;  // (used, and room for it, with offsets only)
 
-    const int warp = threadIdx.x >> 5;
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);  // (uniform to the compiler)
     const int lane = threadIdx.x & 31;
     const int rank = S > 1 ? static_cast<int>(cluster_ctarank()) : 0;
 
     if (warp == 0) {
-        // one barrier a lane: full, empty, conv of a stage; then the others
+        // one stage's barriers a lane; then the others
         if (lane < stages) {
             mbar_init(smem_u32(&full[lane]), 1);
             mbar_init(smem_u32(&empty[lane]), 1);
-            if (C::kConv) mbar_init(smem_u32(&conv[lane]), C::kConvWarps / 2);
         } else if (lane >= 16 && lane < 18) {
             mbar_init(smem_u32(&tfull[lane - 16]), 1);
             mbar_init(smem_u32(&tempty[lane - 16]), C::kEpiWarps);
@@ -622,7 +540,6 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
 
     if (warp == 0) {
         // ---------------------------------------------------- producer ----
-        if (elect_one()) {
         int stage = 0;
         uint32_t phase = 0;
         bool aborted = false;
@@ -631,9 +548,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
         // MN-major products.
         const auto load_p = [&](const RowsItem& w, int kb, int st, int blocks) {
             const uint32_t dst = ring + st * C::kStageBytes, fb = smem_u32(&full[st]);
-            if constexpr (C::kConv) {
-                tma_load_4d(dst + C::kPBytes + C::kQBytes, &tmP, fb, w.p0, w.row0 + kb * C::kBK, 0, 0);
-            } else if constexpr (C::kPMn) {
+            if constexpr (C::kPMn) {
                 const int r = C::kWeight ? w.row0 + kb * C::kBK : kb * C::kBK;
                 const int z = C::kWeight ? 0 : w.e;
                 if (p.p_whole)
@@ -663,42 +578,46 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
         };
         bool waited = !p.early;
         for (int item = first; item < total && !aborted; item += stride) {
-            const RowsItem w = tile_of(item);
+            const RowsItem w = uniform(tile_of(item));
             int kb0, kb1;
             share(w, kb0, kb1);
             const int blocks = blocks_of(w);
             const int boxes = (w.cnt + C::kQBox - 1) / C::kQBox;
-            const int p_bytes = C::kConv ? C::kSub * C::kRawBytes
-                                         : (C::kPMn && !p.p_whole ? blocks * C::kSubBytes : C::kPBytes);
+            const int p_bytes = C::kPMn && !p.p_whole ? blocks * C::kSubBytes : C::kPBytes;
             const int q_bytes = C::kQMn && p.q_whole ? C::kQBytes : boxes * C::kQBoxBytes;
             const uint32_t tx = static_cast<uint32_t>(p_bytes + q_bytes);
             int kb = kb0;
             if (!waited) {
                 // the first ring-full: features now, rows once the kernel before has finished
                 const int ahead = kb1 - kb0 < stages ? kb1 - kb0 : stages;
-                for (int i = 0; i < ahead; ++i) {
-                    mbar_arrive_expect_tx(smem_u32(&full[i]), tx);
-                    load_p(w, kb0 + i, i, blocks);
-                }
+                if (elect_one())
+                    for (int i = 0; i < ahead; ++i) {
+                        mbar_arrive_expect_tx(smem_u32(&full[i]), tx);
+                        load_p(w, kb0 + i, i, blocks);
+                    }
+                __syncwarp();
                 grid_dependency_wait();
                 waited = true;
-                for (int i = 0; i < ahead; ++i) {
-                    load_q(w, kb0 + i, i, boxes);
-                    issued |= 1u << i;
-                }
+                if (elect_one())
+                    for (int i = 0; i < ahead; ++i) load_q(w, kb0 + i, i, boxes);
+                __syncwarp();
+                issued = (1u << ahead) - 1u;
                 kb += ahead;
                 stage = ahead;
                 if (stage == stages) stage = 0, phase = 1u;
             }
             for (; kb < kb1; ++kb) {
-                if (!wait_bounded(smem_u32(&empty[stage]), phase ^ 1u, abort_flag, p.timeout_ns,
-                                  (blockIdx.x << 8) | 0x10u | stage)) {
+                if (!wait_bounded_warp(smem_u32(&empty[stage]), phase ^ 1u, abort_flag, p.timeout_ns,
+                                       (blockIdx.x << 8) | 0x10u | stage)) {
                     aborted = true;
                     break;
                 }
-                mbar_arrive_expect_tx(smem_u32(&full[stage]), tx);
-                load_p(w, kb, stage, blocks);
-                load_q(w, kb, stage, boxes);
+                if (elect_one()) {
+                    mbar_arrive_expect_tx(smem_u32(&full[stage]), tx);
+                    load_p(w, kb, stage, blocks);
+                    load_q(w, kb, stage, boxes);
+                }
+                __syncwarp();
                 issued |= 1u << stage;
                 issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
                 if (++stage == stages) stage = 0, phase ^= 1u;
@@ -708,11 +627,10 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
         // Tail: every stage filled has been released, so no MMA commit arrives
         // on this CTA's barriers after it exits.
         for (int i = 0; i < stages && !aborted; ++i) {
-            if (!wait_bounded(smem_u32(&empty[stage]), phase ^ 1u, abort_flag, p.timeout_ns,
-                              (blockIdx.x << 8) | 0x50u | stage))
+            if (!wait_bounded_warp(smem_u32(&empty[stage]), phase ^ 1u, abort_flag, p.timeout_ns,
+                                   (blockIdx.x << 8) | 0x50u | stage))
                 break;
             if (++stage == stages) stage = 0, phase ^= 1u;
-        }
         }
     } else if (warp == 1) {
         // -------------------------------------------------- MMA issuer ----
@@ -724,7 +642,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
         const uint64_t qdesc = C::kQMn ? smem_desc_sw128(ring + C::kPBytes, C::kAtomBytes, 1024)
                                        : smem_desc_sw128(ring + C::kPBytes, 16, 1024);
         for (int item = first; item < total && !aborted; item += stride) {
-            const RowsItem w = tile_of(item);
+            const RowsItem w = uniform(tile_of(item));
             int kb0, kb1;
             share(w, kb0, kb1);
             if (kb0 == kb1) continue;  // nothing to sum: the epilogue writes zeros
@@ -734,8 +652,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
             const uint32_t idesc = __shfl_sync(0xffffffffu, p.idesc | (static_cast<uint32_t>(n >> 3) << 17), 0);
             // stage st, k-block kb: operands in shared memory
             const auto ready = [&](int st, uint32_t ph) {
-                // (kConv: the converters waited for the stage's copies before they arrived)
-                return wait_bounded_warp(smem_u32(C::kConv ? &conv[st] : &full[st]), ph, abort_flag, p.timeout_ns,
+                return wait_bounded_warp(smem_u32(&full[st]), ph, abort_flag, p.timeout_ns,
                                          (blockIdx.x << 8) | 0x30u | st);
             };
             // The sum ends inside an MMA step of the last k-block: the step's
@@ -746,7 +663,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                 if (!C::kWeight || (valid & 15) == 0) return;
                 uint8_t* base = smem + st * C::kStageBytes;
                 const int extra = 16 - (valid & 15);
-                const int pa = C::kConv ? 0 : 2 * blocks;
+                const int pa = 2 * blocks;
                 for (int i = lane; i < (pa + (n + 63) / 64) * extra * 8; i += 32) {
                     const int a = i / (extra * 8), r = valid + (i / 8) % extra;
                     uint8_t* atom = base + (a < pa ? a * C::kAtomBytes : C::kPBytes + (a - pa) * C::kAtomBytes);
@@ -866,7 +783,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
             }
             acc_phase ^= 1u;
         }
-    } else if (warp >= 2 && warp < C::kFirstConv) {
+    } else if (warp >= 2 && warp < 2 + C::kEpiWarps) {
         // ---------------------------------------------------- epilogue ----
         const int quarter = warp & 3;
         const int group = (warp - 2) >> 2;  // the two groups of four warps take 32 columns in turn
@@ -1008,44 +925,6 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
             }
             if (!empty_sum) acc_phase ^= 1u;
         }
-    } else if (C::kConv && warp >= C::kFirstConv) {
-        // -------------------------------------------------- converters ----
-        const int conv_group = (warp - C::kFirstConv) >> 2;
-        const int ct = (static_cast<int>(threadIdx.x) - 32 * C::kFirstConv) & (kConvThreads - 1);
-        int stage = 0, turn = 0;
-        uint32_t phase = 0;
-        bool ok = true;
-        for (int item = first; item < total && ok; item += stride) {
-            const RowsItem w = tile_of(item);
-            int kb0, kb1;
-            share(w, kb0, kb1);
-            // the scales are fetched a turn ahead: their latency is several conversions long
-            float ahead[ConvRegs<C>::kPerBlock];
-            conv_scales<C>(p, w.row0 + (kb0 + (turn ^ conv_group)) * C::kBK, w.rend, ct, ahead);
-            for (int kb = kb0; kb < kb1; ++kb, turn ^= 1) {
-                if (turn == conv_group) {
-                    ConvRegs<C> g;
-#pragma unroll
-                    for (int u = 0; u < g.kPerBlock; ++u) g.s[u] = ahead[u];
-                    conv_scales<C>(p, w.row0 + (kb + 2) * C::kBK, w.rend, ct, ahead);
-                    if (!wait_bounded_warp(smem_u32(&full[stage]), phase, abort_flag, p.timeout_ns,
-                                           (blockIdx.x << 8) | 0xA0u | stage)) {
-                        ok = false;
-                        break;
-                    }
-                    uint8_t* st = smem + stage * C::kStageBytes;
-                    conv_codes<C>(st + C::kPBytes + C::kQBytes, ct, g);
-                    if (p.bf16)
-                        conv_write<C, true>(st, ct, g);
-                    else
-                        conv_write<C, false>(st, ct, g);
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(&conv[stage]));
-                }
-                if (++stage == stages) stage = 0, phase ^= 1u;
-            }
-        }
     }
     __syncwarp();
     tc_fence_before();
@@ -1053,8 +932,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
     if (*abort_flag) {
         // Some role gave up.  Before shared and tensor memory are released,
         // let this CTA's own copies land and its MMAs retire.
-        // (`issued` is zero in every thread but the producer; elect_one picks
-        // the same lane of the converged warp that issued the MMAs)
+        // (`issued` is zero outside the producer's warp; elect_one picks the same
+        // lane of the converged warp that issued the MMAs)
         for (int s = 0; s < stages; ++s)
             if (issued & (1u << s)) drain_wait(smem_u32(&full[s]), (issued_parity >> s) & 1u);
         __syncwarp();

@@ -949,6 +949,41 @@ tcg_status quantize_rows(const void* src, int8_t* dst, float* scale, long long r
     return launch_quantize_rows<T, kRowThreads, true>(src, dst, scale, rows, k, sms, st);
 }
 
+template <class T, int kCodes>
+tcg_status launch_dequantize_rows(const int8_t* src, const float* scale, void* dst, long long rows, int k, int sms,
+                                  cudaStream_t st)
+{
+    const long long steps = rows * (k / kCodes);
+    long long blocks = (steps + kRowThreads - 1) / kRowThreads;
+    const long long cap = static_cast<long long>(sms) * 16;
+    if (blocks > cap) blocks = cap;
+    cudaLaunchConfig_t cfg;
+    std::memset(&cfg, 0, sizeof cfg);
+    cudaLaunchAttribute attr[1];
+    std::memset(attr, 0, sizeof attr);
+    cfg.gridDim = dim3(static_cast<unsigned>(blocks), 1, 1);
+    cfg.blockDim = dim3(kRowThreads, 1, 1);
+    cfg.stream = st;
+    cfg.attrs = attr;
+    if (pdl_enabled()) {
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.numAttrs = 1;
+    }
+    const cudaError_t e =
+        cudaLaunchKernelEx(&cfg, dequantize_rows_kernel<T, kCodes>, src, scale, static_cast<T*>(dst), rows, k);
+    return e == cudaSuccess ? TCG_SUCCESS : cuda_fail(e);
+}
+
+template <class T>
+tcg_status dequantize_rows(const int8_t* src, const float* scale, void* dst, long long rows, int k, int sms,
+                           cudaStream_t st)
+{
+    if (k % 16 == 0 && aligned16(src) && aligned16(dst))
+        return launch_dequantize_rows<T, 16>(src, scale, dst, rows, k, sms, st);
+    return launch_dequantize_rows<T, 1>(src, scale, dst, rows, k, sms, st);
+}
+
 }  // namespace
 
 extern "C" {
@@ -974,6 +1009,24 @@ tcg_status tcg_quantize_rows_s8(const void* src, tcg_dtype type, int8_t* dst, fl
     if (type == TCG_F32) return quantize_rows<float>(src, dst, scale, rows, k, dev->sms, st);
     if (type == TCG_F16) return quantize_rows<__half>(src, dst, scale, rows, k, dev->sms, st);
     return quantize_rows<__nv_bfloat16>(src, dst, scale, rows, k, dev->sms, st);
+}
+
+tcg_status tcg_dequantize_rows_s8(const int8_t* src, const float* scale, void* dst, tcg_dtype type, long long rows,
+                                  int k, void* stream)
+{
+    if (type != TCG_F32 && type != TCG_F16 && type != TCG_BF16) return TCG_ERR_ARG;
+    if (rows < 0 || k < 0) return TCG_ERR_SHAPE;
+    if (rows == 0 || k == 0) return TCG_SUCCESS;
+    if (!src || !scale || !dst) return TCG_ERR_ARG;
+    if ((reinterpret_cast<uintptr_t>(scale) & 3u) || reinterpret_cast<uintptr_t>(dst) % (type == TCG_F32 ? 4u : 2u))
+        return TCG_ERR_ALIGN;
+    DeviceState* dev;
+    const tcg_status s = device_state(&dev);
+    if (s != TCG_SUCCESS) return s;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (type == TCG_F32) return dequantize_rows<float>(src, scale, dst, rows, k, dev->sms, st);
+    if (type == TCG_F16) return dequantize_rows<__half>(src, scale, dst, rows, k, dev->sms, st);
+    return dequantize_rows<__nv_bfloat16>(src, scale, dst, rows, k, dev->sms, st);
 }
 
 }  // extern "C"

@@ -16,7 +16,8 @@ def test_empty_results_succeed_without_a_device():
     assert L().tcg_gemm_s8_scaled(None, None, None, 1, 0, 8, 16, 1, None, None, None, None) == OK
     assert L().tcg_gemm_s8_grouped(None, None, None, 1, None, 1, 8, 0, 16, None, None, None, 1, None) == OK
     assert L().tcg_gemm_16_grouped(None, None, 1, None, 1, None, 1, 0, 8, 8, 1, 0, None) == OK
-    assert L().tcg_gemm_16_grouped_wgrad(None, None, None, 1, None, 1, None, 0, 4, 8, 8, None) == OK
+    assert L().tcg_gemm_16_grouped_wgrad(None, None, 1, None, 1, None, 0, 4, 8, 8, None) == OK
+    assert L().tcg_dequantize_rows_s8(None, None, None, 1, 4, 0, None) == OK
     assert L().tcg_linear_s8(None, 1, None, None, 1, 0, 8, 16, None, None, None, 0, None) == OK
 
 
@@ -31,6 +32,16 @@ def test_quantize_rows_refusals():
     assert f(18, 0, 16, 16, 4, 8, None) == ALIGN
     assert f(17, 1, 16, 16, 4, 8, None) == ALIGN
     assert f(16, 0, 16, 18, 4, 8, None) == ALIGN
+
+
+def test_dequantize_rows_refusals():
+    f = L().tcg_dequantize_rows_s8  # codes scale dst type rows k stream
+    ok = [16, 16, 16, 1, 4, 8, None]
+    for i, v, st in ((3, 3, ARG), (4, -1, SHAPE), (5, -1, SHAPE), (0, None, ARG), (1, None, ARG), (2, None, ARG),
+                     (1, 18, ALIGN), (2, 17, ALIGN)):
+        args = list(ok)
+        args[i] = v
+        assert f(*args) == st, (i, v)
 
 
 def test_int8_product_refusals():
@@ -83,17 +94,13 @@ def test_16_bit_refusals():
     kn = list(ok)
     kn[10], kn[8] = 0, 12
     assert f(*kn) == SHAPE  # N of a K x N operand
-    w = L().tcg_gemm_16_grouped_wgrad  # dC A scale type dB type offsets groups M N K stream
-    ok = [16, 16, None, 1, 16, 1, 16, 2, 4, 8, 16, None]
-    for i, v, st in ((3, 0, ARG), (5, 3, ARG), (0, None, ARG), (1, None, ARG), (4, None, ARG), (7, 1025, SHAPE),
-                     (9, 4, SHAPE), (10, 12, SHAPE), (8, -1, SHAPE), (0, 24, ALIGN), (1, 24, ALIGN), (4, 17, ALIGN),
-                     (2, 18, ALIGN)):
+    w = L().tcg_gemm_16_grouped_wgrad  # dC A type dB type offsets groups M N K stream
+    ok = [16, 16, 1, 16, 1, 16, 2, 4, 8, 16, None]
+    for i, v, st in ((2, 0, ARG), (4, 3, ARG), (0, None, ARG), (1, None, ARG), (3, None, ARG), (6, 1025, SHAPE),
+                     (8, 4, SHAPE), (9, 12, SHAPE), (7, -1, SHAPE), (0, 24, ALIGN), (1, 24, ALIGN), (3, 17, ALIGN)):
         args = list(ok)
         args[i] = v
         assert w(*args) == st, (i, v)
-    codes = list(ok)
-    codes[2], codes[10] = 16, 24
-    assert w(*codes) == SHAPE  # rows of codes are 16 bytes
 
 
 def test_python_surface_refuses_cpu_tensors_and_wrong_types():

@@ -114,6 +114,15 @@ def test_quantize_rows_leading_axes_and_ties():
     assert q.shape == (3, 0) and s.tolist() == [0, 0, 0]
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("shape", [(1, 1), (3, 33), (2, 5, 64), (700, 528), (5, 20000), (1300, 2048)])
+def test_dequantize_rows_rounds_once(shape, dtype):
+    g = gen(sum(shape))
+    q, s = codes(g, *shape), torch.rand(shape[:-1], generator=g, device=DEV) * 0.1
+    got = T().dequantize_rows_int8(q, s, dtype)
+    assert torch.equal(got, (q.float() * s[..., None]).to(dtype))
+
+
 @pytest.mark.parametrize("value", [float("inf"), float("nan")])
 @pytest.mark.parametrize("k", [48, 41])
 def test_quantize_rows_not_finite_stays_visible(value, k):

@@ -23,6 +23,9 @@ def test_quantize_and_int8_products():
     refuse("contiguous", T.quantize_rows_int8, z(8, 8).t()[:, ::2])
     refuse("float32, float16", T.quantize_rows_int8, z(4, 8, dtype=i8))
     refuse("at least one axis", T.quantize_rows_int8, z())
+    refuse("CUDA int8", T.dequantize_rows_int8, z(4, 8), z(4, dtype=f32))
+    refuse("scales must have shape", T.dequantize_rows_int8, z(4, 8, dtype=i8), z(8, dtype=f32))
+    refuse("dtype must be", T.dequantize_rows_int8, z(4, 8, dtype=i8), z(4, dtype=f32), i8)
     a, b, sa, sb = z(4, 16, dtype=i8), z(6, 16, dtype=i8), z(4, dtype=f32), z(6, dtype=f32)
     refuse("must be int8", T.gemm_int8_scaled, z(4, 16), b, sa, sb)
     refuse("cols must equal", T.gemm_int8_scaled, a, z(6, 32, dtype=i8), sa, sb)
@@ -70,7 +73,7 @@ def test_16_bit_products_and_layers():
     refuse("number of groups", T.gemm_grouped_wgrad, z(4, 8), a, o[:1])
     refuse("save must be", T.linear, a, b[0], save="fp8")
     refuse("multiple of 8", T.linear, z(4, 12), z(8, 12))
-    refuse("multiple of 8", T.linear, z(4, 24), z(8, 24), save="int8")
+    refuse("multiple of 8", T.linear, z(4, 20), z(8, 20), save="int8")
     refuse("N must be", T.linear, a, z(12, 16))
     refuse("must not be empty", T.linear, z(4, 0), z(8, 0))
     refuse("must be contiguous", T.linear, z(16, 4).t(), b[0])
