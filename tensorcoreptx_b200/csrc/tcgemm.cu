@@ -910,7 +910,7 @@ tcg_status tcg_quantize_absmax_s4(const float* src, int8_t* dst_packed, int rows
 
 namespace {
 
-template <class T, int kGroup, bool kVec>
+template <class T, int kGroup, int kVecs>
 tcg_status launch_quantize_rows(const void* src, int8_t* dst, float* scale, long long rows, int k, int sms,
                                 cudaStream_t st)
 {
@@ -931,22 +931,25 @@ tcg_status launch_quantize_rows(const void* src, int8_t* dst, float* scale, long
         attr[0].val.programmaticStreamSerializationAllowed = 1;
         cfg.numAttrs = 1;
     }
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, quantize_rows_kernel<T, kGroup, kVec>, static_cast<const T*>(src),
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, quantize_rows_kernel<T, kGroup, kVecs>, static_cast<const T*>(src),
                                              dst, scale, rows, k);
     return e == cudaSuccess ? TCG_SUCCESS : cuda_fail(e);
 }
 
-// A warp per row while the row fits its registers (one pass, no block
-// barrier) and there are rows enough for every SM; a block per row otherwise.
+// A warp per row where it fits a warp's registers and there are rows enough for
+// every SM (two warps each); a block per row otherwise.
 template <class T>
 tcg_status quantize_rows(const void* src, int8_t* dst, float* scale, long long rows, int k, int sms, cudaStream_t st)
 {
     constexpr int kN = 16 / sizeof(T);
     const bool vec = k % kN == 0 && aligned16(src) && (reinterpret_cast<uintptr_t>(dst) % kN) == 0;
-    if (!vec) return launch_quantize_rows<T, kRowThreads, false>(src, dst, scale, rows, k, sms, st);
-    if (k <= 32 * kRowVecs * kN && rows >= 4LL * sms)
-        return launch_quantize_rows<T, 32, true>(src, dst, scale, rows, k, sms, st);
-    return launch_quantize_rows<T, kRowThreads, true>(src, dst, scale, rows, k, sms, st);
+    if (!vec) return launch_quantize_rows<T, kRowThreads, 0>(src, dst, scale, rows, k, sms, st);
+    const int per_lane = (k / kN + 31) / 32;
+    if (rows >= 2LL * sms) {
+        if (per_lane <= 8) return launch_quantize_rows<T, 32, 8>(src, dst, scale, rows, k, sms, st);
+        if (per_lane <= 16) return launch_quantize_rows<T, 32, 16>(src, dst, scale, rows, k, sms, st);
+    }
+    return launch_quantize_rows<T, kRowThreads, 8>(src, dst, scale, rows, k, sms, st);
 }
 
 template <class T, int kCodes>

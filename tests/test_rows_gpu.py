@@ -106,6 +106,21 @@ def test_quantize_rows_bit_exact(rows, k, dtype):
     assert np.array_equal(s.cpu().numpy().view(np.uint32), sh.view(np.uint32))
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_quantize_rows_every_code_and_size(dtype):
+    """All codes, halves between them, signed zeros, and rows from the smallest to the largest magnitudes."""
+    base = torch.cat([torch.arange(-254, 255), torch.tensor([0.0, -0.0, 253.5])]).to(F32) / 2
+    tiny = torch.finfo(dtype).smallest_normal
+    sizes = [1.0, 2.0, 0.75, 1e-3, 100.0, float(tiny), float(tiny) * 2 ** -7, float(torch.finfo(dtype).max) / 128]
+    x = torch.stack([(base.double() * s).to(dtype) for s in sizes]).to(DEV)
+    for k in (512, 504, 511):
+        y = x[:, :k].contiguous() if k < 512 else x
+        q, s = T().quantize_rows_int8(y)
+        qh, sh = quantize_host(y)
+        assert np.array_equal(s.cpu().numpy().view(np.uint32), sh.view(np.uint32))
+        assert np.array_equal(q.cpu().numpy(), qh), k
+
+
 def test_quantize_rows_leading_axes_and_ties():
     x = torch.tensor([[[254.0, 1.0, 3.0, -1.0, -5.0, 0.0]], [[0.0] * 6]], device=DEV)  # scale 2: halves tie away
     q, s = T().quantize_rows_int8(x)
