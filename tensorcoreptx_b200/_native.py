@@ -68,6 +68,7 @@ SIGNATURES = {
 }
 
 _lib = None
+_torch = None
 _lock = threading.Lock()
 
 
@@ -101,6 +102,21 @@ def lib():
                 fn.argtypes = args
             _lib = L
     return _lib
+
+
+def torch_binding():
+    """The torch binding (csrc/tcg_torch.cpp), loaded once; ImportError if it is
+    not built."""
+    global _torch
+    if _torch is None:
+        import torch  # noqa: F401  (its libraries first)
+        lib()
+        path = os.path.join(HERE, "_tcg_torch.so")
+        if not os.path.exists(path):
+            raise ImportError(f"{path} is missing: build it with `python -m tensorcoreptx_b200.build`")
+        from . import _tcg_torch
+        _torch = _tcg_torch
+    return _torch
 
 
 def check(fn: str, status: int):

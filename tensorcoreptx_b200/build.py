@@ -5,6 +5,8 @@
 
 Outputs, next to this file:
     libtcgemm.so                 the C ABI of include/tcgemm.h (all kernels)
+    _tcg_torch.so                the torch binding of the calls that are bound by
+                                 the host when small (csrc/tcg_torch.cpp, g++)
     libtcgemm_compat_f16.so      reference-compatible C++ `launch_kernel` +
     libtcgemm_compat_s8.so       `Solver*` per precision (include/tcgemm_compat.h),
     libtcgemm_compat_s4.so       one per precision as the reference links one
@@ -15,6 +17,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -27,6 +30,7 @@ COMMON = ARCH + ["-O3", "-std=c++17", "-lineinfo", "-shared", "-Xcompiler", "-fP
                  "-I" + INCLUDE]
 
 LIB = os.path.join(HERE, "libtcgemm.so")
+TORCH = os.path.join(HERE, "_tcg_torch.so")
 COMPAT = {p: os.path.join(HERE, f"libtcgemm_compat_{p}.so") for p in ("f16", "s8", "s4")}
 
 
@@ -80,6 +84,18 @@ def _compile(names, force, verbose):
     return objects
 
 
+def _torch_command(out):
+    import torch
+    root = os.path.dirname(torch.__file__)
+    include = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+               os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include"), sysconfig.get_paths()["include"], INCLUDE]
+    return (["g++", "-O2", "-std=c++17", "-shared", "-fPIC",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] + ["-I" + i for i in include] +
+            _sources("tcg_torch.cpp") + ["-o", out, "-L" + os.path.join(root, "lib"), "-ltorch", "-ltorch_cpu",
+                                         "-ltorch_python", "-lc10", "-lc10_cuda", "-L" + HERE, "-ltcgemm",
+                                         "-Wl,-rpath,$ORIGIN"])
+
+
 def build(force: bool = False, verbose: bool = True) -> list[str]:
     deps = _deps()
     built = []
@@ -93,6 +109,9 @@ def build(force: bool = False, verbose: bool = True) -> list[str]:
             _run([NVCC] + COMMON + ["-D" + defines[prec]] + _sources("compat.cu") +
                  ["-L" + HERE, "-ltcgemm", "-Xlinker", "-rpath=$ORIGIN", "-o", out], verbose)
             built.append(out)
+    if force or _stale(TORCH, [LIB] + sorted(_includes(*_sources("tcg_torch.cpp")))):
+        _run(_torch_command(TORCH), verbose)
+        built.append(TORCH)
     return built
 
 
