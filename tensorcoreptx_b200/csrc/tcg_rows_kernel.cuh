@@ -26,7 +26,9 @@
 //     depend on timing).  For few rows, where the weights' bytes bound the
 //     product and every SM has to pull on memory.
 //   kSub = 2: 256 x 256, persistent CTAs, two M = 128 accumulators that fill
-//     the tensor memory.  For many rows, where the tensor cores bound it.
+//     the tensor memory.  Where the number of tiles is known at launch there is
+//     a CTA per tile, and running CTAs take over those that have not started
+//     (cluster launch control), so that groups of different length balance.  For many rows, where the tensor cores bound it.
 //
 // Warps: 0 TMA producer, 1 MMA issuer, 2..9 epilogue (two per
 // tensor-memory lane quarter).  Every wait on an mbarrier is bounded (tcg_wait.cuh).
@@ -62,6 +64,7 @@ struct RowsParams {
     int split_log2;           // kSub = 1: 1, 2, 4 or 8 CTAs per tile
     int stages;               // ring depth
     int p_whole, q_whole;     // MN-major operands of whole 64-element atoms: one copy a tile and stage
+    int dynamic;              // kSub = 2: a CTA per item, running ones taking over those not started
     int early;                // the M-side operand and the offsets predate the kernel this one follows
     uint32_t idesc;           // instruction descriptor without N
 };
@@ -91,7 +94,8 @@ struct RowsTraits {
     static constexpr int kTmemCols = kSub * kBQ < 32 ? 32 : kSub * kBQ;
     static constexpr int kRedBytes = kBQ * 512;         // split: 128 x kBQ partial sums
     static constexpr int kMaxStages = 12;
-    static constexpr int kBarBytes = 256;
+    static constexpr int kRing = 4;                     // kSub = 2: items on their way to the other roles
+    static constexpr int kBarBytes = 384;
     static constexpr int kScaleBytes = 1024;            // scales of the rows being written out
     // two blocks of 32 x 128 results on their way out; one tile a CTA: in the ring, which is idle by then
     static constexpr int kOutBytes = 8192;
@@ -99,7 +103,7 @@ struct RowsTraits {
     static_assert(!kQMn || kKind == kKindF16, "weight form: 16-bit operands");
     static_assert(!kPMn || kKind == kKindF16, "MN-major features: 16-bit operands");
     static_assert(!kQMn || kBQ % 64 == 0, "whole 64-column atoms");
-    static_assert(8 * (2 * kMaxStages + 5) + 16 <= kBarBytes, "barrier area");
+    static_assert(8 * (2 * kMaxStages + 6 + 2 * kRing) + 8 + 4 * kRing + 16 <= kBarBytes - 16, "barrier area");
     static_assert((kTmemCols & (kTmemCols - 1)) == 0 && kTmemCols <= 512, "TMEM allocation");
     // dynamic shared memory of a launch with a table of `groups` groups
     static constexpr int smem_bytes(int stages, int split, int groups)
@@ -466,8 +470,13 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
     uint64_t* tfull = empty + C::kMaxStages;  // accumulator block h complete
     uint64_t* tempty = tfull + 2;            // accumulator block h read
     uint64_t* drain = tempty + 2;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+    uint64_t* qfull = drain + 1;             // item published
+    uint64_t* qempty = qfull + C::kRing;     // item read by the MMA issuer and every epilogue warp
+    uint64_t* clcbar = qempty + C::kRing;    // cluster launch control has answered
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(clcbar + 1);
     volatile uint32_t* abort_flag = tmem_slot + 1;
+    volatile int* ring_item = reinterpret_cast<volatile int*>(tmem_slot + 2);
+    const uint32_t clc_answer = smem_u32(reinterpret_cast<uint8_t*>(full) + C::kBarBytes - 16);  // 16-byte aligned
     int* bound = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(full) + C::kBarBytes);
     int* cum = bound + p.groups + 3;  // (used, and room for it, with offsets only)
 
@@ -485,7 +494,11 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
             mbar_init(smem_u32(&tempty[lane - 16]), C::kEpiWarps);
         } else if (lane == 18) {
             mbar_init(smem_u32(drain), 1);
+            mbar_init(smem_u32(clcbar), 1);
             *abort_flag = 0u;
+        } else if (lane >= 24 && lane < 24 + C::kRing) {
+            mbar_init(smem_u32(&qfull[lane - 24]), 1);
+            mbar_init(smem_u32(&qempty[lane - 24]), 1 + C::kEpiWarps);
         } else if (lane == 19) {
             tma_prefetch_desc(&tmP);
         } else if (lane == 20) {
@@ -507,7 +520,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
     if (p.offsets && warp == 2) rows_table(p, C::kBQ, bound, cum);
     tc_fence_before();
     __syncthreads();
-    if (S > 1) cluster_sync_all();  // every CTA of the cluster runs before any writes into another
+    if (S > 1) cluster_arrive();  // every CTA of the cluster runs before any writes into another (push_part)
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     const uint32_t ring = smem_u32(smem);
@@ -524,6 +537,25 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
             return rows_tile<C>(p, static_cast<int>(blockIdx.y), tq1, static_cast<int>(blockIdx.z), bound, cum);
         else
             return rows_item<C>(p, item, qtiles, bound, cum);
+    };
+    // Items reach the MMA issuer and the epilogue like this.  Static: every
+    // stride-th item.  Dynamic: whatever the producer has published (-1 at the
+    // end; a wait that gave up ends the role too).
+    const bool dynamic = C::kSub == 2 && p.dynamic;
+    int q = 0;
+    uint32_t qph = 0;
+    const auto next_item = [&](int item) {
+        if (!dynamic) {
+            item = item < 0 ? first : item + stride;
+            return item < total ? item : -1;
+        }
+        if (!wait_bounded_warp(smem_u32(&qfull[q]), qph, abort_flag, p.timeout_ns, (blockIdx.x << 8) | 0x70u | q))
+            return -1;
+        item = ring_item[q];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&qempty[q]));
+        if (++q == C::kRing) q = 0, qph ^= 1u;
+        return item;
     };
     // this CTA's share [kb0, kb1) of a tile's k-blocks
     const auto share = [&](const RowsItem& w, int& kb0, int& kb1) {
@@ -577,7 +609,36 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
             }
         };
         bool waited = !p.early;
-        for (int item = first; item < total && !aborted; item += stride) {
+        bool asked = false;  // an answer of cluster launch control is on its way
+        uint32_t clc_phase = 0;
+        // The item after `item` (-1: none).  Dynamic: publish that one and ask
+        // for the CTA to take over; the answer is read after its loads.
+        const auto publish = [&](int item) {
+            if (!wait_bounded_warp(smem_u32(&qempty[q]), qph ^ 1u, abort_flag, p.timeout_ns,
+                                   (blockIdx.x << 8) | 0x78u | q))
+                return false;
+            if (elect_one()) {
+                ring_item[q] = item;
+                mbar_arrive(smem_u32(&qfull[q]));
+            }
+            __syncwarp();
+            if (++q == C::kRing) q = 0, qph ^= 1u;
+            return true;
+        };
+        for (int item = first < total ? first : -1; !aborted;) {
+            if (dynamic && !publish(item)) {
+                aborted = true;
+                break;
+            }
+            if (item < 0) break;
+            if (dynamic) {
+                if (elect_one()) {
+                    mbar_arrive_expect_tx(smem_u32(clcbar), 16);
+                    clc_try_cancel(clc_answer, smem_u32(clcbar));
+                }
+                __syncwarp();
+                asked = true;
+            }
             const RowsItem w = uniform(tile_of(item));
             int kb0, kb1;
             share(w, kb0, kb1);
@@ -622,7 +683,22 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                 issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
                 if (++stage == stages) stage = 0, phase ^= 1u;
             }
+            if (aborted) break;
+            if (dynamic) {
+                if (!wait_bounded_warp(smem_u32(clcbar), clc_phase, abort_flag, p.timeout_ns,
+                                       (blockIdx.x << 8) | 0x7Cu)) {
+                    aborted = true;
+                    break;
+                }
+                asked = false;
+                clc_phase ^= 1u;
+                int taken = -1;
+                item = clc_query(clc_answer, taken) ? taken : -1;
+            } else {
+                item = item + stride < total ? item + stride : -1;
+            }
         }
+        if (asked) drain_wait(smem_u32(clcbar), clc_phase);  // (aborting: the answer lands in this CTA's memory)
         if (!waited) grid_dependency_wait();
         // Tail: every stage filled has been released, so no MMA commit arrives
         // on this CTA's barriers after it exits.
@@ -641,7 +717,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
         const uint64_t pdesc = C::kPMn ? smem_desc_sw128(ring, C::kAtomBytes, 1024) : smem_desc_sw128(ring, 16, 1024);
         const uint64_t qdesc = C::kQMn ? smem_desc_sw128(ring + C::kPBytes, C::kAtomBytes, 1024)
                                        : smem_desc_sw128(ring + C::kPBytes, 16, 1024);
-        for (int item = first; item < total && !aborted; item += stride) {
+        for (int item = next_item(-1); item >= 0 && !aborted; item = next_item(item)) {
             const RowsItem w = uniform(tile_of(item));
             int kb0, kb1;
             share(w, kb0, kb1);
@@ -791,8 +867,9 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
         uint32_t* stage_out = reinterpret_cast<uint32_t*>(out_area + group * C::kOutBytes);
         uint32_t acc_phase = 0;
         bool lost = false;
+        if (S > 1) cluster_wait();
         if (p.early) grid_dependency_wait();  // the rows' scales, and the output's last readers
-        for (int item = first; item < total && !lost; item += stride) {
+        for (int item = next_item(-1); item >= 0 && !lost; item = next_item(item)) {
             const RowsItem w = tile_of(item);
             int kb0, kb1;
             share(w, kb0, kb1);
@@ -965,7 +1042,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                     scales[t] = rank * per + t < w.cnt && !w.zero ? p.scale_q[w.row0 + rank * per + t] : 0.f;
             }
         }
-        cluster_sync_all();  // every part has arrived
+        if (warp < 2) cluster_wait();  // (the epilogue's warps have)
+        cluster_sync_all();            // every part has arrived
         if (work && t < 256) {
             if (p.out_type == kOutF32)
                 finish<C, float>(p, w, red, scales, rank, t, sp, bias);

@@ -180,6 +180,21 @@ def test_int8_scaled_every_tile_and_split(tile, split):
     check(T().gemm_int8_scaled(A, B, sa, sb, bias, out_dtype=F32), *int8_reference(A, B, sa, sb, bias, F32))
 
 
+@pytest.mark.parametrize("K", [4096, 4112])
+def test_more_tiles_than_sms_taken_over(K):
+    """Long sums in more 256-row tiles than there are SMs, last tiles partial in both directions."""
+    g = gen(K)
+    M, N = 3400, 3336
+    A, B = codes(g, M, K), codes(g, N, K)
+    sa, sb = torch.rand(M, generator=g, device=DEV), torch.rand(N, generator=g, device=DEV)
+    T().set_rows_tile(256, 0)
+    check(T().gemm_int8_scaled(A, B, sa, sb, out_dtype=BF16), *int8_reference(A, B, sa, sb, None, BF16))
+    x, W, dy = randn(g, 2200, 3400, dtype=BF16), randn(g, 3336, 3400, dtype=BF16), randn(g, 2200, 3336, dtype=BF16)
+    check(T().linear(x, W), *product_reference(x, W.t(), BF16, 3400))
+    got = T().gemm_grouped_wgrad(dy, x, offsets_of([0, 2200]))
+    check(got, *wgrad_reference(dy, x, [0, 2200], BF16))
+
+
 def test_int8_scaled_batches():
     g = gen(5)
     b, M, N, K = 3, 37, 65, 96
