@@ -40,6 +40,7 @@ struct RowsCall {
 struct RowsPlan {
     int bq;     // 16, 32, 64, 128 (kSub = 1) or 256 (kSub = 2)
     int split;
+    int chunk;  // k-blocks summed in one go
 };
 
 int ceil_div(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
@@ -68,10 +69,15 @@ RowsPlan choose_plan(const RowsCall& c, bool weight, int kblock, int sms)
     const double mean = static_cast<double>(c.rows) / c.groups;  // rows per group
     const double kb = weight ? (mean + kblock - 1) / kblock : ceil_div(c.R, kblock);
     const double used = c.groups < c.rows ? c.groups : c.rows;   // groups that can have rows
-    RowsPlan best{128, 1};
+    // fp32 results of long 16-bit sums: in chunks of 512, which the tiles of 256
+    // rows have no room for
+    const bool fine = kblock == 64 && c.out_type == kOutF32 && (weight ? c.rows : c.R) > 512;
+    const int chunk = fine ? 8 : 0x7fffffff;
+    RowsPlan best{128, 1, chunk};
     double least = -1;
     for (int bq = weight ? 128 : 16; bq <= 256; bq *= 2) {
         if (forced && bq != forced && !(weight && forced < 128 && bq == 128)) continue;
+        if (!forced && fine && bq == 256) continue;
         const int tile_p = bq == 256 ? 256 : 128;
         double q;  // tiles along q: a ragged group ends half a tile early on average
         if (weight)
@@ -93,7 +99,7 @@ RowsPlan choose_plan(const RowsCall& c, bool weight, int kblock, int sms)
                     std::max(1.0, tiles * split / sms) * kb / split * (bq == 128 ? 0.30 : 0.20);
             if (least < 0 || t < least) {
                 least = t;
-                best = RowsPlan{bq, split};
+                best = RowsPlan{bq, split, chunk};
             }
         }
     }
@@ -101,7 +107,7 @@ RowsPlan choose_plan(const RowsCall& c, bool weight, int kblock, int sms)
 }
 
 template <class C>
-tcg_status launch(const RowsCall& c, int split, int dev, int sms, cudaStream_t st)
+tcg_status launch(const RowsCall& c, int split, int chunk, int dev, int sms, cudaStream_t st)
 {
     static std::atomic<bool> smem_set[host::kDevices];
     auto kern = rows_kernel<C>;
@@ -217,6 +223,7 @@ tcg_status launch(const RowsCall& c, int split, int dev, int sms, cudaStream_t s
     if (C::kSub == 1 && !C::kWeight)  // no more than a CTA's share of the sum: what is left can start the next kernel
         stages = std::max(2, std::min(stages, ceil_div(ceil_div(c.R, C::kBK), split)));
     p.stages = stages;
+    p.chunk = chunk;
     cfg.dynamicSmemBytes = C::smem_bytes(stages, split, table);
     cfg.stream = st;
     cfg.attrs = attr;
@@ -244,11 +251,11 @@ tcg_status run_rows(const RowsCall& c, cudaStream_t st)
     if (s != TCG_SUCCESS) return s;
     const RowsPlan plan = choose_plan(c, false, kKind == kKindF16 ? 64 : 128, sms);
     switch (plan.bq) {
-    case 16: return launch<RowsTraits<kKind, kPMn, false, 1, 16>>(c, plan.split, dev, sms, st);
-    case 32: return launch<RowsTraits<kKind, kPMn, false, 1, 32>>(c, plan.split, dev, sms, st);
-    case 64: return launch<RowsTraits<kKind, kPMn, false, 1, 64>>(c, plan.split, dev, sms, st);
-    case 128: return launch<RowsTraits<kKind, kPMn, false, 1, 128>>(c, plan.split, dev, sms, st);
-    default: return launch<RowsTraits<kKind, kPMn, false, 2, 256>>(c, 1, dev, sms, st);
+    case 16: return launch<RowsTraits<kKind, kPMn, false, 1, 16>>(c, plan.split, plan.chunk, dev, sms, st);
+    case 32: return launch<RowsTraits<kKind, kPMn, false, 1, 32>>(c, plan.split, plan.chunk, dev, sms, st);
+    case 64: return launch<RowsTraits<kKind, kPMn, false, 1, 64>>(c, plan.split, plan.chunk, dev, sms, st);
+    case 128: return launch<RowsTraits<kKind, kPMn, false, 1, 128>>(c, plan.split, plan.chunk, dev, sms, st);
+    default: return launch<RowsTraits<kKind, kPMn, false, 2, 256>>(c, 1, plan.chunk, dev, sms, st);
     }
 }
 
@@ -258,8 +265,8 @@ tcg_status run_weight(const RowsCall& c, cudaStream_t st)
     const tcg_status s = host::device(&dev, &sms);
     if (s != TCG_SUCCESS) return s;
     const RowsPlan plan = choose_plan(c, true, 64, sms);
-    if (plan.bq == 256) return launch<RowsTraits<kKindF16, true, true, 2, 256>>(c, 1, dev, sms, st);
-    return launch<RowsTraits<kKindF16, true, true, 1, 128>>(c, plan.split, dev, sms, st);
+    if (plan.bq == 256) return launch<RowsTraits<kKindF16, true, true, 2, 256>>(c, 1, plan.chunk, dev, sms, st);
+    return launch<RowsTraits<kKindF16, true, true, 1, 128>>(c, plan.split, plan.chunk, dev, sms, st);
 }
 
 bool is_type(tcg_dtype t) { return t == TCG_F32 || t == TCG_F16 || t == TCG_BF16; }

@@ -23,7 +23,10 @@
 //   kSub = 1: 128 features x kBQ rows, one tile per cluster.  The CTAs of a
 //     cluster (1, 2, 4 or 8) split the sum between them and add their parts
 //     through distributed shared memory, in rank order (the result does not
-//     depend on timing).  For few rows, where the weights' bytes bound the
+//     depend on timing).  fp32 results are summed in chunks of 512: the tensor
+//     cores drop the bits that do not fit when they add to an accumulator, an
+//     error that grows with the length of the chain (2.4e-6 of the result at K =
+//     2048, 0.6e-6 in chunks, added with one rounding each).  For few rows, where the weights' bytes bound the
 //     product and every SM has to pull on memory.
 //   kSub = 2: 256 x 256, persistent CTAs, two M = 128 accumulators that fill
 //     the tensor memory.  Where the number of tiles is known at launch there is
@@ -63,6 +66,7 @@ struct RowsParams {
     int out_type;
     int split_log2;           // kSub = 1: 1, 2, 4 or 8 CTAs per tile
     int stages;               // ring depth
+    int chunk;                // kChunks: k-blocks that the tensor cores add up in one go
     int p_whole, q_whole;     // MN-major operands of whole 64-element atoms: one copy a tile and stage
     int dynamic;              // kSub = 2: a CTA per item, running ones taking over those not started
     int early;                // the M-side operand and the offsets predate the kernel this one follows
@@ -88,10 +92,10 @@ struct RowsTraits {
     static constexpr int kQBoxBytes = kQBox * kBK * kElem;
     static constexpr int kEpiWarps = 8;                 // two per quarter of the tensor memory's lanes
     static constexpr int kThreads = 32 * (2 + kEpiWarps);
-    // 16-bit results of a whole tile fit the epilogue's registers
-    static constexpr bool kHold = kSub == 2;
     static constexpr int kPerSm = kSub == 1 ? 2 : 1;  // CTAs per SM that registers are kept for
-    static constexpr int kTmemCols = kSub * kBQ < 32 ? 32 : kSub * kBQ;
+    // kSub = 1 with fp32 sums: two accumulators that take chunks of the sum in turn
+    static constexpr bool kChunks = kSub == 1 && kKind == kKindF16;
+    static constexpr int kTmemCols = kChunks ? 2 * kBQ : (kSub * kBQ < 32 ? 32 : kSub * kBQ);
     static constexpr int kRedBytes = kBQ * 512;         // split: 128 x kBQ partial sums
     static constexpr int kMaxStages = 12;
     static constexpr int kRing = 4;                     // kSub = 2: items on their way to the other roles
@@ -750,7 +754,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
             };
             // the MMAs of k-block kb in stage st into the accumulator blocks of
             // `mask`; a descriptor's low word is an address in 16-byte units
-            const auto issue = [&](int st, int kb, int mask) {
+            const auto issue = [&](int st, int kb, int mask, uint32_t d, bool fresh) {
                 tc_fence_after();
                 // (broadcasts, so that the compiler knows the operands to be uniform)
                 const uint64_t at = static_cast<uint64_t>(__shfl_sync(0xffffffffu, st, 0)) * (C::kStageBytes / 16);
@@ -762,10 +766,10 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                         if (k >= ksteps) break;
                         const uint64_t qd = qdesc + at + k * (C::kQMn ? C::kUmmaK * 8 : 2);
                         const uint64_t pd = pdesc + at + k * (C::kPMn ? C::kUmmaK * 8 : 2);
-                        const uint32_t sum = kb > kb0 || k > 0 ? 1u : 0u;
-                        if (mask & 1) umma<C::kKind>(tmem_base, pd, qd, idesc, sum);
+                        const uint32_t sum = !fresh || k > 0 ? 1u : 0u;
+                        if (mask & 1) umma<C::kKind>(d, pd, qd, idesc, sum);
                         if (C::kSub == 2 && (mask & 2))
-                            umma<C::kKind>(tmem_base + C::kBQ, pd + C::kSubBytes / 16, qd, idesc, sum);
+                            umma<C::kKind>(d + C::kBQ, pd + C::kSubBytes / 16, qd, idesc, sum);
                     }
                 }
                 __syncwarp();
@@ -779,8 +783,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                 if (elect_one()) umma_commit(smem_u32(&tfull[h]));
                 __syncwarp();
             };
-            if (!wait_bounded_warp(smem_u32(&tempty[0]), acc_phase ^ 1u, abort_flag, p.timeout_ns,
-                                   (blockIdx.x << 8) | 0x20u))
+            if (C::kSub == 2 && !wait_bounded_warp(smem_u32(&tempty[0]), acc_phase ^ 1u, abort_flag, p.timeout_ns,
+                                                   (blockIdx.x << 8) | 0x20u))
                 break;
             const int mask = blocks == 2 ? 3 : 1;
             int kb = kb0;
@@ -803,7 +807,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                         break;
                     }
                     if (kb0 + held == kb1 - 1) clear_rest(st, kb0 + held);
-                    issue(st, kb0 + held, 1);
+                    issue(st, kb0 + held, 1, tmem_base, held == 0);
                     ++held;
                     next();
                     free1 = __all_sync(0xffffffffu, mbar_try_wait(smem_u32(&tempty[1]), acc_phase ^ 1u));
@@ -813,7 +817,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                                                  (blockIdx.x << 8) | 0x21u))
                     break;
                 for (; kb < kb0 + held; ++kb) {
-                    issue(stage, kb, mask & 2);
+                    issue(stage, kb, mask & 2, tmem_base, kb == kb0);
                     release();
                 }
                 const int last = kb1 - kb < stages ? kb1 - kb : stages;
@@ -822,7 +826,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                         aborted = true;
                         break;
                     }
-                    issue(stage, kb, mask);
+                    issue(stage, kb, mask, tmem_base, kb == kb0);
                     release();
                 }
                 if (aborted) break;
@@ -834,28 +838,42 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                         break;
                     }
                     if (kb + i == kb1 - 1) clear_rest(st, kb + i);
-                    issue(st, kb + i, 1);
+                    issue(st, kb + i, 1, tmem_base, kb + i == kb0);
                     next();
                 }
                 if (aborted) break;
                 complete(0);
                 for (; kb < kb1; ++kb) {
-                    issue(stage, kb, mask & 2);
+                    issue(stage, kb, mask & 2, tmem_base, kb == kb0);
                     release();
                 }
                 complete(1);
             } else {
+                // Chunks of the sum into two accumulators in turn: the epilogue
+                // takes one to its registers while the other fills.
+                int part = 0;  // k-blocks of the chunk so far
+                int buf = 0;
                 for (; kb < kb1; ++kb) {
+                    if (part == 0 && !wait_bounded_warp(smem_u32(&tempty[buf]), acc_phase ^ 1u, abort_flag,
+                                                        p.timeout_ns, (blockIdx.x << 8) | 0x20u | buf)) {
+                        aborted = true;
+                        break;
+                    }
                     if (!ready(stage, phase)) {
                         aborted = true;
                         break;
                     }
                     if (kb == kb1 - 1) clear_rest(stage, kb);
-                    issue(stage, kb, 1);
+                    issue(stage, kb, 1, tmem_base + buf * C::kBQ, part == 0);
                     release();
+                    if (++part == p.chunk || kb == kb1 - 1) {
+                        complete(buf);
+                        part = 0;
+                        buf ^= 1;
+                        if (buf == 0) acc_phase ^= 1u;
+                    }
                 }
                 if (aborted) break;
-                complete(0);
             }
             acc_phase ^= 1u;
         }
@@ -876,19 +894,16 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
             const bool empty_sum = kb0 == kb1;
             const long long row = C::kWeight ? static_cast<long long>(w.e) * p.Q + w.q0 : w.row0;
             float sp = 0.f, bias = 0.f;  // of this lane's feature in the current block
-            // wait for block h of the accumulators
-            const auto begin = [&](int h) {
-                if (!empty_sum) {
-                    // (the four warps of a group agree on the outcome: none is
-                    // left waiting at a barrier that another has given up)
-                    const bool ok = wait_bounded_warp(smem_u32(&tfull[h]), acc_phase, abort_flag, p.timeout_ns,
-                                                      (blockIdx.x << 8) | 0x40u | h);
-                    if (!named_barrier_and(2 + group, 128, ok)) {
-                        lost = true;
-                        return;
-                    }
-                    tc_fence_after();
-                }
+            // wait for accumulator (kSub = 2: block) h; the four warps of a group
+            // agree on the outcome: none is left waiting at a barrier that
+            // another has given up
+            const auto await = [&](int h, uint32_t parity) {
+                const bool ok = wait_bounded_warp(smem_u32(&tfull[h]), parity, abort_flag, p.timeout_ns,
+                                                  (blockIdx.x << 8) | 0x40u | h);
+                if (!named_barrier_and(2 + group, 128, ok)) lost = true;
+                tc_fence_after();
+            };
+            const auto channel = [&](int h) {
                 const int f = w.p0 + h * 128 + quarter * 32 + lane;
                 if (C::kKind == kKindI8 && S == 1 && f < p.P && !w.zero) {
                     const long long at = static_cast<long long>(w.e) * p.P + f;
@@ -896,27 +911,18 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                     bias = p.bias_p ? p.bias_p[at] : 0.f;
                 }
             };
-            // columns c .. c + 31 of block h
-            const auto load = [&](int h, int c, uint32_t (&v)[32]) {
-                if (empty_sum) {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = 0u;
-                } else {
-                    tmem_ld_32x32b_x32(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
-                                           static_cast<uint32_t>(h * C::kBQ + c),
-                                       v);
-                }
+            // 32 columns of the accumulators from column c on
+            const auto load = [&](int c, uint32_t (&v)[32]) {
+                tmem_ld_32x32b_x32(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(c), v);
             };
-            const auto load_wait = [&]() {
-                if (!empty_sum) tmem_ld_wait();
-            };
-            const auto finish_load = [&](int c, uint32_t (&v)[32], float (&x)[32]) {
+            const auto rows_scales = [&](int c) {
                 if (C::kKind == kKindI8) {  // the rows' scales, for every lane to read
                     __syncwarp();
                     warp_scales[lane] = !w.zero && c + lane < w.cnt ? p.scale_q[w.row0 + c + lane] : 0.f;
                     __syncwarp();
                 }
-                load_wait();
+            };
+            const auto results = [&](const uint32_t (&v)[32], float (&x)[32]) {
 #pragma unroll
                 for (int j = 0; j < 32; ++j) {
                     // int8: the int32 sum, rounded to fp32 once, times both scales, plus the bias
@@ -927,7 +933,6 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                 }
             };
             const auto release = [&](int h) {
-                if (empty_sum) return;
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&tempty[h]));
@@ -936,7 +941,73 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                 return OutBlock{p.out, row + c, p.P, w.p0 + h * 128, min(32, w.cnt - c),
                                 min(128, p.P - w.p0 - h * 128), p.aligned_out != 0};
             };
-            if (C::kHold && p.out_type != kOutF32 && p.aligned_out) {
+            const auto store = [&](const float (&x)[32], const OutBlock& o) {
+                if (p.out_type == kOutF32) {
+                    store_block32(x, o, stage_out, quarter, lane, 2 + group);
+                } else {
+                    uint32_t words[16];
+                    pack_block(x, p.out_type == kOutBF16, words);
+                    if (o.aligned)
+                        store_block16(words, o, stage_out, quarter, lane, 2 + group);
+                    else
+                        store_rows16(words, o, quarter, lane);
+                }
+            };
+            if constexpr (C::kSub == 1) {
+                // The sum, chunk by chunk, in this thread's registers.
+                constexpr int kMine = (C::kBQ + 63) / 64;  // blocks of 32 columns
+                uint32_t sum[kMine][32];
+#pragma unroll
+                for (int i = 0; i < kMine; ++i)
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) sum[i][j] = 0u;
+                channel(0);
+                int buf = 0;
+                uint32_t parity = 0;
+                for (int kb = kb0; kb < kb1;) {
+                    await(buf, parity);
+                    if (lost) break;
+#pragma unroll
+                    for (int i = 0; i < kMine; ++i) {
+                        const int c = 32 * group + 64 * i;
+                        if (c >= w.cnt) continue;
+                        uint32_t v[32];
+                        load(buf * C::kBQ + c, v);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            sum[i][j] = C::kChunks ? __float_as_uint(__uint_as_float(sum[i][j]) + __uint_as_float(v[j]))
+                                                   : v[j];
+                    }
+                    release(buf);
+                    if (kb1 - kb <= p.chunk) break;
+                    kb += p.chunk;
+                    buf ^= 1;
+                    if (buf == 0) parity ^= 1u;
+                }
+                if (lost) break;
+#pragma unroll
+                for (int i = 0; i < kMine; ++i) {
+                    const int c = 32 * group + 64 * i;
+                    if (c >= w.cnt) continue;
+                    if (S > 1) {
+                        push_part<C>(sum[i], red, rank, p.split_log2, c, min(32, w.cnt - c), quarter * 32 + lane);
+                        continue;
+                    }
+                    float x[32];
+                    rows_scales(c);
+                    results(sum[i], x);
+                    store(x, block_of(0, c));
+                }
+            } else if (empty_sum) {
+                // rows outside the groups, a group without rows: zeros
+                const float x[32] = {};
+                for (int h = 0; h < C::kSub; ++h)
+                    for (int c = 32 * group; c < w.cnt; c += 64) {
+                        const OutBlock o = block_of(h, c);
+                        if (o.features > 0) store(x, o);
+                    }
+            } else if (p.out_type != kOutF32 && p.aligned_out) {
                 // Both blocks into registers (128 words a thread) before any
                 // store: the accumulators are free for the next tile after
                 // about 3000 cycles instead of the 11000 that the stores of
@@ -945,7 +1016,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     if (lost) break;
-                    begin(h);
+                    await(h, acc_phase);
+                    channel(h);
                     if (lost) break;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -953,8 +1025,10 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                         if (c < w.cnt) {
                             uint32_t v[32];
                             float x[32];
-                            load(h, c, v);
-                            finish_load(c, v, x);
+                            load(h * C::kBQ + c, v);
+                            rows_scales(c);
+                            tmem_ld_wait();
+                            results(v, x);
                             pack_block(x, p.out_type == kOutBF16, held[h][i]);
                         }
                     }
@@ -971,31 +1045,20 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                     }
             } else {
                 for (int h = 0; h < C::kSub; ++h) {
-                    begin(h);
+                    await(h, acc_phase);
+                    channel(h);
                     if (lost) break;
 #pragma unroll 1
                     for (int c = 32 * group; c < w.cnt; c += 64) {
-                        uint32_t v[32];
-                        load(h, c, v);
-                        if (C::kSub == 1 && S > 1) {
-                            load_wait();
-                            push_part<C>(v, red, rank, p.split_log2, c, min(32, w.cnt - c), quarter * 32 + lane);
-                            continue;
-                        }
-                        float x[32];
-                        finish_load(c, v, x);
                         const OutBlock o = block_of(h, c);
                         if (o.features <= 0) break;  // (uniform) the second half of the last tile along P
-                        if (p.out_type == kOutF32) {
-                            store_block32(x, o, stage_out, quarter, lane, 2 + group);
-                        } else {
-                            uint32_t words[16];
-                            pack_block(x, p.out_type == kOutBF16, words);
-                            if (o.aligned)
-                                store_block16(words, o, stage_out, quarter, lane, 2 + group);
-                            else
-                                store_rows16(words, o, quarter, lane);
-                        }
+                        uint32_t v[32];
+                        float x[32];
+                        load(h * C::kBQ + c, v);
+                        rows_scales(c);
+                        tmem_ld_wait();
+                        results(v, x);
+                        store(x, o);
                     }
                     release(h);
                 }
