@@ -35,6 +35,8 @@ struct RowsCall {
     const float *scale_q, *scale_p, *bias_p;
     int zero_rest;
     int early;
+    const void* x;  // rows that the product quantises itself
+    int x_type;
 };
 
 struct RowsPlan {
@@ -144,8 +146,10 @@ tcg_status launch(const RowsCall& c, int split, int chunk, int dev, int sms, cud
     else
         s = host::encode_4d(&mp, dt, c.pside, k_major(P, G, C::kTileP), swz);
     if (s == TCG_SUCCESS)
-        s = C::kWeight ? host::encode_4d(&mq, dt, c.qside, atoms(Q, M, 1, q_whole, C::kBQ / 64), swz)
-                       : host::encode_4d(&mq, dt, c.qside, k_major(M, 1, C::kBQ), swz);
+        s = C::kOwn ? TCG_SUCCESS
+            : C::kWeight ? host::encode_4d(&mq, dt, c.qside, atoms(Q, M, 1, q_whole, C::kBQ / 64), swz)
+                         : host::encode_4d(&mq, dt, c.qside, k_major(M, 1, C::kBQ), swz);
+    if (C::kOwn) mq = mp;  // (no copies of rows)
     mqb = mq;
     if (s == TCG_SUCCESS && !C::kWeight && C::kBQ > C::kQBox)
         s = host::encode_4d(&mqb, dt, c.qside, k_major(M, 1, C::kQBox), swz);
@@ -168,6 +172,10 @@ tcg_status launch(const RowsCall& c, int split, int chunk, int dev, int sms, cud
     p.ptiles = ceil_div(c.P, C::kTileP);
     p.qtiles = ceil_div(C::kWeight ? c.Q : p.rows_per_group, C::kBQ);
     p.zero_rest = c.zero_rest;
+    p.x = c.x;
+    p.x_type = c.x_type;
+    p.own_blocks = C::kOwn ? ceil_div(ceil_div(c.R, C::kBK), split) : 0;
+    const auto smem_for = [&](int n) { return C::smem_bytes(n, split, c.offsets ? c.groups : 0, p.own_blocks); };
     const int out_bytes = c.out_type == kOutF32 ? 4 : 2;
     p.aligned_out = (static_cast<long long>(c.P) * out_bytes) % 16 == 0 && (reinterpret_cast<uintptr_t>(c.out) & 15u) == 0;
     p.out_type = c.out_type;
@@ -175,7 +183,6 @@ tcg_status launch(const RowsCall& c, int split, int chunk, int dev, int sms, cud
     p.early = c.early;
     p.p_whole = p_whole;
     p.q_whole = q_whole;
-    const int table = c.offsets ? c.groups : 0;
     const uint32_t fmt = C::kKind == kKindI8 ? 1u : (c.bf16 ? 1u : 0u);
     p.idesc = make_idesc(C::kKind == kKindI8 ? 2u : 1u, fmt, fmt, C::kQMn, 128, 0) | (C::kPMn ? 1u << 15 : 0u);
 
@@ -215,16 +222,16 @@ tcg_status launch(const RowsCall& c, int split, int chunk, int dev, int sms, cud
     // Ring depth: all of shared memory for one CTA per SM; half of it, so that
     // one CTA's start and end overlap another's loads, where there are more
     // CTAs than SMs (kSub = 1).
-    const int room = C::kSub == 1 && items * split > sms && 2 * C::smem_bytes(2, split, table) <= most - 2048
+    const int room = C::kSub == 1 && items * split > sms && 2 * smem_for(2) <= most - 2048
                          ? (most - 2048) / 2
                          : most;
-    int stages = (room - C::smem_bytes(0, split, table)) / C::kStageBytes;
+    int stages = (room - smem_for(0)) / C::kStageBytes;
     if (stages > C::kMaxStages) stages = C::kMaxStages;
     if (C::kSub == 1 && !C::kWeight)  // no more than a CTA's share of the sum: what is left can start the next kernel
         stages = std::max(2, std::min(stages, ceil_div(ceil_div(c.R, C::kBK), split)));
     p.stages = stages;
     p.chunk = chunk;
-    cfg.dynamicSmemBytes = C::smem_bytes(stages, split, table);
+    cfg.dynamicSmemBytes = smem_for(stages);
     cfg.stream = st;
     cfg.attrs = attr;
     if (split > 1) {
@@ -269,6 +276,15 @@ tcg_status run_weight(const RowsCall& c, cudaStream_t st)
     return launch<RowsTraits<kKindF16, true, true, 1, 128>>(c, plan.split, plan.chunk, dev, sms, st);
 }
 
+// Whether a product of `rows` ungrouped rows quantises them itself: few rows, and
+// a CTA's share of them fits its shared memory.
+bool owns_rows(const RowsCall& c, int sms, RowsPlan* plan)
+{
+    if (c.offsets || c.groups != 1 || c.rows > kOwnRows) return false;
+    *plan = choose_plan(c, false, 128, sms);
+    return plan->bq == 16 && ceil_div(ceil_div(c.R, 128), plan->split) <= kOwnBlocks;
+}
+
 bool is_type(tcg_dtype t) { return t == TCG_F32 || t == TCG_F16 || t == TCG_BF16; }
 bool misaligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) % n) != 0; }
 unsigned size_of(tcg_dtype t) { return t == TCG_F32 ? 4u : 2u; }
@@ -289,15 +305,10 @@ tcg_status check(int M, int N, int K, int groups, const int32_t* offsets, long l
     return TCG_SUCCESS;
 }
 
-tcg_status gemm_s8(const int8_t* A, const int8_t* B, void* C, tcg_dtype c_type, const int32_t* offsets, int groups,
-                   int M, int N, int K, const float* scale_a, const float* scale_b, const float* bias, int zero_rest,
-                   int early, cudaStream_t st)
+// The call that multiplies rows A (codes, or null: x quantised on the way).
+RowsCall s8_call(const int8_t* A, const int8_t* B, void* C, tcg_dtype c_type, const int32_t* offsets, int groups, int M,
+                 int N, int K, const float* scale_a, const float* scale_b, const float* bias, int zero_rest)
 {
-    if (!A || !B || !C || !scale_a || !scale_b) return TCG_ERR_ARG;
-    if (K == 0 || K % 16 != 0) return TCG_ERR_SHAPE;
-    if (misaligned(A, 16) || misaligned(B, 16) || misaligned(C, size_of(c_type)) || misaligned(scale_a, 4) ||
-        misaligned(scale_b, 4) || misaligned(bias, 4))
-        return TCG_ERR_ALIGN;
     RowsCall c;
     std::memset(&c, 0, sizeof c);
     c.pside = B;
@@ -313,6 +324,19 @@ tcg_status gemm_s8(const int8_t* A, const int8_t* B, void* C, tcg_dtype c_type, 
     c.scale_p = scale_b;
     c.bias_p = bias;
     c.zero_rest = zero_rest;
+    return c;
+}
+
+tcg_status gemm_s8(const int8_t* A, const int8_t* B, void* C, tcg_dtype c_type, const int32_t* offsets, int groups,
+                   int M, int N, int K, const float* scale_a, const float* scale_b, const float* bias, int zero_rest,
+                   int early, cudaStream_t st)
+{
+    if (!A || !B || !C || !scale_a || !scale_b) return TCG_ERR_ARG;
+    if (K == 0 || K % 16 != 0) return TCG_ERR_SHAPE;
+    if (misaligned(A, 16) || misaligned(B, 16) || misaligned(C, size_of(c_type)) || misaligned(scale_a, 4) ||
+        misaligned(scale_b, 4) || misaligned(bias, 4))
+        return TCG_ERR_ALIGN;
+    RowsCall c = s8_call(A, B, C, c_type, offsets, groups, M, N, K, scale_a, scale_b, bias, zero_rest);
     c.early = early && host::dependent_launch();
     return run_rows<kKindI8, false>(c, st);
 }
@@ -374,12 +398,25 @@ tcg_status tcg_linear_s8_grouped(const void* x, tcg_dtype x_type, const int8_t* 
     tcg_status s = check(M, N, K, groups, offsets, static_cast<long long>(M) * N, &done);
     if (s != TCG_SUCCESS || done) return s;
     // everything is checked before the first launch
-    if (!x || !B || !C || !scale_b || !workspace) return TCG_ERR_ARG;
+    if (!x || !B || !C || !scale_b) return TCG_ERR_ARG;
     if (K == 0 || K % 16 != 0) return TCG_ERR_SHAPE;
-    if (workspace_bytes < tcg_linear_s8_workspace_size(M, K)) return TCG_ERR_WORKSPACE;
-    if (misaligned(workspace, 256) || misaligned(x, size_of(x_type)) || misaligned(B, 16) ||
-        misaligned(C, size_of(c_type)) || misaligned(scale_b, 4) || misaligned(bias, 4))
+    if (misaligned(x, size_of(x_type)) || misaligned(B, 16) || misaligned(C, size_of(c_type)) ||
+        misaligned(scale_b, 4) || misaligned(bias, 4))
         return TCG_ERR_ALIGN;
+    if (!offsets && groups == 1 && M <= kOwnRows && !misaligned(x, 16)) {
+        int dev, sms;
+        if ((s = host::device(&dev, &sms)) != TCG_SUCCESS) return s;
+        RowsCall c = s8_call(nullptr, B, C, c_type, nullptr, 1, M, N, K, nullptr, scale_b, bias, 0);
+        c.x = x;
+        c.x_type = x_type;
+        RowsPlan plan;
+        if (owns_rows(c, sms, &plan))
+            return launch<RowsTraits<kKindI8, false, false, 1, 16, true>>(c, plan.split, plan.chunk, dev, sms,
+                                                                          static_cast<cudaStream_t>(stream));
+    }
+    if (!workspace) return TCG_ERR_ARG;
+    if (workspace_bytes < tcg_linear_s8_workspace_size(M, K)) return TCG_ERR_WORKSPACE;
+    if (misaligned(workspace, 256)) return TCG_ERR_ALIGN;
     int8_t* codes = static_cast<int8_t*>(workspace);
     float* scale = reinterpret_cast<float*>(codes + round256(static_cast<size_t>(M) * K));
     s = tcg_quantize_rows_s8(x, x_type, codes, scale, M, K, stream);

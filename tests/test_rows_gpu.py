@@ -88,9 +88,10 @@ def quantize_host(x):
     """The definition in IEEE single precision, on the host."""
     x = x.float().cpu().numpy()
     scale = (np.abs(x).max(-1) / np.float32(127)).astype(np.float32)
-    with np.errstate(divide="ignore"):
+    with np.errstate(divide="ignore", over="ignore", invalid="ignore"):
         inv = np.where(scale > 0, np.float32(1) / scale, np.float32(0)).astype(np.float32)
-    q = np.clip((x * inv[..., None]).astype(np.float32), np.float32(-127), np.float32(127))
+        q = np.clip((x * inv[..., None]).astype(np.float32), np.float32(-127), np.float32(127))
+    q[np.isnan(q)] = 0  # 0 x inf: the scale is too small to have an inverse
     return np.where(q >= 0, np.floor(q + np.float32(0.5)), np.ceil(q - np.float32(0.5))).astype(np.int8), scale
 
 
@@ -227,6 +228,33 @@ def test_linear_int8_is_quantise_then_product(shape, dtype):
     qh, sh = quantize_host(x.view(-1, shape[-1]))
     ref, bound = int8_reference(torch.from_numpy(qh).to(DEV), B, torch.from_numpy(sh).to(DEV), sb, bias, dtype)
     check(y.view(ref.shape), ref, bound)
+
+
+@pytest.mark.parametrize("split", [0, 1, 2, 4, 8])
+@pytest.mark.parametrize("M,N,K", [(1, 1, 16), (2, 130, 48), (3, 300, 1040), (4, 1000, 4112), (1, 4099, 16384),
+                                   (4, 257, 40960)])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_linear_int8_of_few_rows(M, N, K, dtype, split):
+    """Rows that the product quantises itself: the two-step result, bit for bit."""
+    g = gen(M + K)
+    x, B = randn(g, M, K, dtype=dtype), codes(g, N, K)
+    x[M - 1] *= 0 if M == 3 else 1
+    sb, bias = torch.rand(N, generator=g, device=DEV) * 0.01, randn(g, N)
+    T().set_rows_tile(16 if split else 0, split)
+    y = T().linear_int8(x, B, sb, bias)
+    q, s = T().quantize_rows_int8(x)
+    assert torch.equal(y, T().gemm_int8_scaled(q, B, s, sb, bias, out_dtype=dtype))
+    # at an address that is not a multiple of 16 bytes, too
+    z = torch.empty(M * K + 1, dtype=dtype, device=DEV)[1:].view(M, K)
+    z.copy_(x)
+    assert torch.equal(T().linear_int8(z, B, sb, bias), y)
+
+
+def test_linear_int8_of_few_rows_not_finite():
+    x = torch.ones(3, 64, device=DEV)
+    x[1, 5] = float("nan")
+    y = T().linear_int8(x, torch.ones(40, 64, dtype=torch.int8, device=DEV), torch.ones(40, device=DEV))
+    assert torch.isnan(y[1]).all() and torch.isfinite(y[[0, 2]]).all()
 
 
 GROUPS = [
