@@ -167,8 +167,8 @@ tcg_status tcg_linear_s8(const void* x, tcg_dtype x_type, const int8_t* B, void*
  * offsets: groups + 1 ascending row bounds on the device (0 < groups <=
  * TCG_MAX_GROUPS), any of the groups empty; they are clamped to be ascending
  * and within 0 .. M.  Rows of C outside every group are set to zero
- * (zero_rest != 0) or left as they are.  NULL offsets: `groups` groups of
- * M / groups rows each (M % groups == 0).
+ * (zero_rest != 0) or left as they are.  NULL offsets: `groups` (at most
+ * 65535) groups of M / groups rows each (M % groups == 0).
  * tcg_gemm_16_grouped: A and B fp16 or bf16 (`type`), fp32 sums, C rounded once
  * to c_type; B is groups x N x K (TCG_B_NK) or groups x K x N (TCG_B_KN); K % 8
  * == 0 (and N % 8 == 0 for TCG_B_KN).  The gradient by A is the same product

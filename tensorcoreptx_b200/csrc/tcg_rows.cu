@@ -299,7 +299,7 @@ tcg_status check(int M, int N, int K, int groups, const int32_t* offsets, long l
         *done = true;
         return TCG_SUCCESS;
     }
-    if (groups == 0 || groups > TCG_MAX_GROUPS) return TCG_ERR_SHAPE;
+    if (groups == 0 || groups > (offsets ? TCG_MAX_GROUPS : 65535)) return TCG_ERR_SHAPE;  // (table; grid)
     if (!offsets && M % groups != 0) return TCG_ERR_SHAPE;
     if (misaligned(offsets, 4)) return TCG_ERR_ALIGN;
     return TCG_SUCCESS;

@@ -20,21 +20,28 @@
 // per-channel scales are one register a lane.
 //
 // Two sizes of tile:
-//   kSub = 1: 128 features x kBQ rows, one tile per cluster.  The CTAs of a
-//     cluster (1, 2, 4 or 8) split the sum between them and add their parts
-//     through distributed shared memory, in rank order (the result does not
-//     depend on timing).  fp32 results are summed in chunks of 512: the tensor
-//     cores drop the bits that do not fit when they add to an accumulator, an
-//     error that grows with the length of the chain (2.4e-6 of the result at K =
-//     2048, 0.6e-6 in chunks, added with one rounding each).  For few rows, where the weights' bytes bound the
-//     product and every SM has to pull on memory.
-//   kSub = 2: 256 x 256, persistent CTAs, two M = 128 accumulators that fill
-//     the tensor memory.  Where the number of tiles is known at launch there is
-//     a CTA per tile, and running CTAs take over those that have not started
-//     (cluster launch control), so that groups of different length balance.  For many rows, where the tensor cores bound it.
+//   kSub = 1: 128 features x kBQ rows, one tile per cluster, for few rows, where
+//     the weights' bytes bound the product and every SM has to pull on memory.
+//     The CTAs of a cluster (1, 2, 4 or 8) split the sum between them and add
+//     their parts through distributed shared memory, in rank order (the result
+//     does not depend on timing).  fp32 results are summed in chunks of 512: the
+//     tensor cores drop the bits that do not fit when they add to an
+//     accumulator, an error that grows with the length of the chain (2.4e-6 of
+//     the result at K = 2048; 0.6e-6 in chunks, added with one rounding each).
+//   kSub = 2: 256 x 256, two M = 128 accumulators that fill the tensor memory,
+//     for many rows, where the tensor cores bound the product.  Persistent CTAs
+//     take every so manieth tile; or, where the number of tiles is known at
+//     launch and tiles are long, there is a CTA per tile and running CTAs take
+//     over those that have not started (cluster launch control).
 //
-// Warps: 0 TMA producer, 1 MMA issuer, 2..9 epilogue (two per
-// tensor-memory lane quarter).  Every wait on an mbarrier is bounded (tcg_wait.cuh).
+// Warps: 0 TMA producer, 1 MMA issuer, 2..9 epilogue (two per tensor-memory lane
+// quarter).  Every wait on an mbarrier is bounded (tcg_wait.cuh).
+//
+// What bounds it (B200): one row of 4096 x 4096 int8 6.2 us, of which loading,
+// multiplying and adding up are 3 and the rest launch and synchronisation;
+// experts' weights of 64 x 2048 x 4096 int8 at 6.0 TB/s of 6.5; int8 16384 x 8192
+// x 8192 2.8-2.9 POPS and bf16 8192 x 8192 x 4096 1.48-1.57 PFLOP/s under the
+// power limit, as cuBLAS.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -119,8 +126,8 @@ struct RowsTraits {
     // dynamic shared memory of a launch with a table of `groups` groups
     static constexpr int smem_bytes(int stages, int split, int groups, int own_blocks)
     {
-        return 1024 + stages * kStageBytes + kOutArea + own_blocks * kQBytes + (split > 1 ? kRedBytes : 0) + kScaleBytes + kBarBytes +
-               8 * (groups + 3);
+        return 1024 + stages * kStageBytes + kOutArea + own_blocks * kQBytes + (split > 1 ? kRedBytes : 0) +
+               kScaleBytes + kBarBytes + 8 * (groups + 3);
     }
 };
 
@@ -288,9 +295,9 @@ __device__ __forceinline__ uint32_t pack16(float a, float b)
 // warps of one epilogue group as one feature a lane, out to memory with whole
 // 128-byte lines a warp: through 8 KB of shared memory, 16 x 128 words at a
 // time -- for 16-bit results a word is one feature of two rows.  (Straight from
-// the registers a warp's store is 64 bytes of one row, and the stores, not the
-// tensor cores, bound products with K < 8192: int8 8192 x 8192 x 1024 took
-// 101 us that way.)
+// the registers a warp's store is 64 bytes of one row.  With whole lines and
+// the accumulators freed early, see below: bf16 8192 x 8192 x 4096 394 -> 368 us,
+// weight gradients of 16 groups of 1024 rows, 4096 x 2048, 257 -> 228.)
 struct OutBlock {
     void* out;
     long long row;   // first row
@@ -660,9 +667,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
         int stage = 0;
         uint32_t phase = 0;
         bool aborted = false;
-        // One copy per operand and stage wherever the layout allows: a copy costs
-        // this thread about 100 cycles, and eight of them per stage bounded the
-        // MN-major products.
+        // One copy per operand and stage wherever the layout allows.
         const auto load_p = [&](const RowsItem& w, int kb, int st, int blocks) {
             const uint32_t dst = ring + st * C::kStageBytes, fb = smem_u32(&full[st]);
             if constexpr (C::kPMn) {
@@ -846,7 +851,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
 #pragma unroll
                     for (int k = 0; k < C::kBK / C::kUmmaK; ++k) {
                         if (k >= ksteps) break;
-                        const uint64_t qd = qdesc + (C::kOwn ? (kb - kb0) * (C::kQBytes / 16) : at) + k * (C::kQMn ? C::kUmmaK * 8 : 2);
+                        const uint64_t qat = C::kOwn ? static_cast<uint64_t>((kb - kb0) * (C::kQBytes / 16)) : at;
+                        const uint64_t qd = qdesc + qat + k * (C::kQMn ? C::kUmmaK * 8 : 2);
                         const uint64_t pd = pdesc + at + k * (C::kPMn ? C::kUmmaK * 8 : 2);
                         const uint32_t sum = !fresh || k > 0 ? 1u : 0u;
                         if (mask & 1) umma<C::kKind>(d, pd, qd, idesc, sum);

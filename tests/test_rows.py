@@ -51,7 +51,7 @@ def test_int8_product_refusals():
     assert f(16, 16, 16, 1, 4, 4, 16, -1, 16, 16, None, None) == SHAPE
     assert f(16, 16, 16, 1, 4, 4, 24, 1, 16, 16, None, None) == SHAPE
     assert f(16, 16, 16, 1, 4, 4, 0, 1, 16, 16, None, None) == SHAPE
-    assert f(16, 16, 16, 1, 4, 4, 16, 1025, 16, 16, None, None) == SHAPE
+    assert f(16, 16, 16, 1, 4, 4, 16, 65536, 16, 16, None, None) == SHAPE
     assert f(16, 16, 16, 1, 1 << 30, 4, 16, 4, 16, 16, None, None) == SHAPE  # 2^32 rows
     for i in (0, 1, 2, 8, 9):
         args = [16, 16, 16, 1, 4, 4, 16, 1, 16, 16, None, None]

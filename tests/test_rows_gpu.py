@@ -206,6 +206,16 @@ def test_int8_scaled_batches():
         check(C[i], *int8_reference(A[i], B[i], sa[i], sb[i], bias[i], BF16))
 
 
+def test_int8_scaled_more_batches_than_groups():
+    g = gen(6)
+    b, M, N, K = 1500, 3, 17, 32
+    A, B = codes(g, b, M, K), codes(g, b, N, K)
+    sa, sb = torch.rand(b, M, generator=g, device=DEV), torch.rand(b, N, generator=g, device=DEV)
+    C = T().gemm_int8_scaled(A, B, sa, sb, out_dtype=F32)
+    prod = torch.bmm(A.double(), B.double().transpose(1, 2)) * sa.double()[..., None] * sb.double()[:, None]
+    check(C, prod, rounded(prod, 3.1 * U * prod.abs(), F32))
+
+
 def test_int8_largest_sums_are_exact():
     K = 8192  # 127 * 127 * 8192 needs 27 bits: rounded to fp32 once
     A = torch.full((2, K), 127, dtype=torch.int8, device=DEV)
@@ -318,6 +328,38 @@ def test_grouped(sizes, lead, rows, layout, dtype, out):
         return ref
 
     check(got, per_group(edges, rows, one), bound)
+
+
+@pytest.mark.parametrize("tile", [16, 128, 256])
+@pytest.mark.parametrize("N,out", [(1, None), (77, None), (331, F32), (515, None)])
+def test_grouped_into_rows_of_odd_length(tile, N, out):
+    g = gen(N)
+    sizes, rows, K = [33, 0, 200, 7], 244, 136
+    edges = edges_of(sizes)
+    A, B = randn(g, rows, K, dtype=F16), randn(g, 4, N, K, dtype=F16)
+    T().set_rows_tile(tile, 0)
+    got = T().gemm_grouped(A, B, offsets_of(edges), out_dtype=out)
+    bound = torch.zeros(rows, N, dtype=torch.float64, device=DEV)
+
+    def one(e, a, z):
+        ref, bnd = product_reference(A[a:z], B[e].t(), got.dtype, K)
+        bound[a:z] = bnd
+        return ref
+
+    check(got, per_group(edges, rows, one), bound)
+
+
+@pytest.mark.parametrize("K", [520, 2048, 4104])
+@pytest.mark.parametrize("rows", [20, 700])
+def test_fp32_results_of_long_sums(K, rows):
+    """Chunks of 512: the error of a chain is counted over 512 terms, and one rounding per chunk."""
+    g = gen(K)
+    A, B = randn(g, rows, K, dtype=F16), randn(g, 1, 256, K, dtype=F16)
+    got = T().gemm_grouped(A, B, offsets_of([0, rows]), out_dtype=F32)
+    ref = A.double() @ B[0].double().t()
+    total = A.double().abs() @ B[0].double().abs().t()
+    check(got, ref, rounded(ref, (2 * U * 512 + U * (K // 512 + 1)) * total, F32))
+    assert (got.double() - ref).norm() / ref.norm() < 1e-6
 
 
 @pytest.mark.parametrize("tile", [16, 32, 64, 128, 256])
@@ -555,6 +597,20 @@ def test_linear_gradient_of_an_expanded_output_and_partial_needs():
     assert not T().linear(x.detach(), W.detach()).requires_grad
 
 
+def test_linear_refuses_a_second_differentiation():
+    x, W = torch.randn(8, 64, device=DEV).to(BF16).requires_grad_(True), torch.randn(16, 64, device=DEV).to(BF16)
+    W.requires_grad_(True)
+    y = T().linear(x, W)
+    first = torch.autograd.grad(y.float().square().sum(), (x, W), create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiate twice"):
+        first[0].float().sum().backward()
+    y = T().linear(x, W)
+    with torch.no_grad():
+        W.add_(1.0)  # what the backward pass needs has changed
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        torch.autograd.grad(y.sum(), x)
+
+
 def test_linear_keeps_half_the_bytes():
     x = torch.randn(4096, 2048, device=DEV).to(BF16).requires_grad_(True)
     W = torch.randn(64, 2048, device=DEV).to(BF16).requires_grad_(True)
@@ -650,6 +706,31 @@ def test_serving_step_captured_and_replayed():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, want[i])
+
+
+def test_layers_on_another_stream_and_from_another_thread():
+    """A step whose forward runs on a side stream, its backward from another host thread."""
+    import threading
+    t = T()
+    g = gen(25)
+    x, W = randn(g, 200, 128, dtype=BF16).requires_grad_(True), randn(g, 136, 128, dtype=BF16).requires_grad_(True)
+    dy = randn(g, 200, 136, dtype=BF16)
+    want = torch.autograd.grad(t.linear(x, W, save="int8"), (x, W), dy)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    got = []
+    with torch.cuda.stream(side):
+        y = t.linear(x, W, save="int8")
+
+    def backward():
+        with torch.cuda.stream(side):
+            got.extend(torch.autograd.grad(y, (x, W), dy))
+
+    th = threading.Thread(target=backward)
+    th.start()
+    th.join()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 def test_calls_on_two_streams_do_not_share_anything():
