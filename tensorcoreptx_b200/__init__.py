@@ -6,6 +6,8 @@ tensor cores, behind the reference's entry points:
 
 * Python: ``gemm_fp16(A, B)``, ``gemm_int8(A, BT)`` (bindings/bindings_*.cpp)
   plus ``gemm_int4``;
+* language-model operators: row-scaled int8 products, products grouped by
+  expert, layers with 8-bit checkpoints (rows.py);
 * C ABI: include/tcgemm.h (libtcgemm.so);
 * C++: ``launch_kernel`` / ``Solver*`` (include/tcgemm_compat.h,
   libtcgemm_compat_{f16,s8,s4}.so).
