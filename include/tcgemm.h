@@ -151,9 +151,10 @@ tcg_status tcg_dequantize_rows_s8(const int8_t* src, const float* scale, void* d
  * aligned, C aligned to its element; M and N arbitrary.
  * tcg_linear_s8 quantises its left operand itself (tcg_quantize_rows_s8) into
  * `workspace` (tcg_linear_s8_workspace_size bytes, 256-byte aligned, not
- * shared by calls that may overlap), then multiplies.  Few rows (up to three, at
- * a 16-byte aligned x) are usually quantised inside the product, with the same
- * result, and then leave the workspace alone. */
+ * shared by calls that may overlap), then multiplies.  Products of up to four
+ * rows (and 24576 of their values, 2^27 products, x 16-byte aligned) quantise
+ * them on the way, with the same result, and leave the workspace alone; without
+ * one, calls that need it return TCG_ERR_WORKSPACE and launch nothing. */
 tcg_status tcg_gemm_s8_scaled(const int8_t* A, const int8_t* B, void* C, tcg_dtype c_type, int M, int N, int K,
                               int batches, const float* scale_a, const float* scale_b, const float* bias,
                               void* stream);

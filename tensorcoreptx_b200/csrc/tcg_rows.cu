@@ -10,6 +10,7 @@
 #include <cstring>
 
 #include "../../include/tcgemm.h"
+#include "tcg_fewrows.cuh"
 #include "tcg_host.h"
 #include "tcg_rows_kernel.cuh"
 
@@ -35,8 +36,6 @@ struct RowsCall {
     const float *scale_q, *scale_p, *bias_p;
     int zero_rest;
     int early;
-    const void* x;  // rows that the product quantises itself
-    int x_type;
 };
 
 struct RowsPlan {
@@ -146,10 +145,8 @@ tcg_status launch(const RowsCall& c, int split, int chunk, int dev, int sms, cud
     else
         s = host::encode_4d(&mp, dt, c.pside, k_major(P, G, C::kTileP), swz);
     if (s == TCG_SUCCESS)
-        s = C::kOwn ? TCG_SUCCESS
-            : C::kWeight ? host::encode_4d(&mq, dt, c.qside, atoms(Q, M, 1, q_whole, C::kBQ / 64), swz)
-                         : host::encode_4d(&mq, dt, c.qside, k_major(M, 1, C::kBQ), swz);
-    if (C::kOwn) mq = mp;  // (no copies of rows)
+        s = C::kWeight ? host::encode_4d(&mq, dt, c.qside, atoms(Q, M, 1, q_whole, C::kBQ / 64), swz)
+                       : host::encode_4d(&mq, dt, c.qside, k_major(M, 1, C::kBQ), swz);
     mqb = mq;
     if (s == TCG_SUCCESS && !C::kWeight && C::kBQ > C::kQBox)
         s = host::encode_4d(&mqb, dt, c.qside, k_major(M, 1, C::kQBox), swz);
@@ -172,10 +169,7 @@ tcg_status launch(const RowsCall& c, int split, int chunk, int dev, int sms, cud
     p.ptiles = ceil_div(c.P, C::kTileP);
     p.qtiles = ceil_div(C::kWeight ? c.Q : p.rows_per_group, C::kBQ);
     p.zero_rest = c.zero_rest;
-    p.x = c.x;
-    p.x_type = c.x_type;
-    p.own_blocks = C::kOwn ? ceil_div(ceil_div(c.R, C::kBK), split) : 0;
-    const auto smem_for = [&](int n) { return C::smem_bytes(n, split, c.offsets ? c.groups : 0, p.own_blocks); };
+    const auto smem_for = [&](int n) { return C::smem_bytes(n, split, c.offsets ? c.groups : 0); };
     const int out_bytes = c.out_type == kOutF32 ? 4 : 2;
     p.aligned_out = (static_cast<long long>(c.P) * out_bytes) % 16 == 0 && (reinterpret_cast<uintptr_t>(c.out) & 15u) == 0;
     p.out_type = c.out_type;
@@ -276,13 +270,49 @@ tcg_status run_weight(const RowsCall& c, cudaStream_t st)
     return launch<RowsTraits<kKindF16, true, true, 1, 128>>(c, plan.split, plan.chunk, dev, sms, st);
 }
 
-// Whether a product of `rows` ungrouped rows quantises them itself: few rows, and
-// a CTA's share of them fits its shared memory.
-bool owns_rows(const RowsCall& c, int sms, RowsPlan* plan)
+template <class T, int kM, int kF>
+tcg_status launch_few(const FewParams& p, int sms, cudaStream_t st)
 {
-    if (c.offsets || c.groups != 1 || c.rows > kOwnRows) return false;
-    *plan = choose_plan(c, false, 128, sms);
-    return plan->bq == 16 && ceil_div(ceil_div(c.R, 128), plan->split) <= kOwnBlocks;
+    static_assert(kFewCodes <= 40 * 1024, "shared memory without opting in");
+    cudaLaunchConfig_t cfg;
+    std::memset(&cfg, 0, sizeof cfg);
+    cudaLaunchAttribute attr[1];
+    std::memset(attr, 0, sizeof attr);
+    const int blocks = ceil_div(p.n, kFewWarps * kF);
+    cfg.gridDim = dim3(static_cast<unsigned>(blocks < 2 * sms ? blocks : 2 * sms), 1, 1);
+    cfg.blockDim = dim3(kFewThreads, 1, 1);
+    cfg.dynamicSmemBytes = static_cast<size_t>(kM) * p.k;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    if (host::dependent_launch()) {
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.numAttrs = 1;
+    }
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, few_rows_kernel<T, kM, kF>, p);
+    return e == cudaSuccess ? TCG_SUCCESS : host::fail(e);
+}
+
+template <class T>
+tcg_status run_few(const FewParams& p, int rows, cudaStream_t st)
+{
+    int dev, sms;
+    const tcg_status s = host::device(&dev, &sms);
+    if (s != TCG_SUCCESS) return s;
+    const bool pair = p.n >= kFewPair;
+    switch (rows) {
+    case 1: return launch_few<T, 1, 1>(p, sms, st);
+    case 2: return pair ? launch_few<T, 2, 2>(p, sms, st) : launch_few<T, 2, 1>(p, sms, st);
+    case 3: return pair ? launch_few<T, 3, 2>(p, sms, st) : launch_few<T, 3, 1>(p, sms, st);
+    default: return pair ? launch_few<T, 4, 2>(p, sms, st) : launch_few<T, 4, 1>(p, sms, st);
+    }
+}
+
+// Whether few_rows_kernel takes a product of ungrouped rows.
+bool few_rows(int M, int N, int K)
+{
+    return M <= kFewRows && static_cast<long long>(M) * K <= kFewCodes &&
+           static_cast<long long>(M) * N * K <= kFewWork;
 }
 
 bool is_type(tcg_dtype t) { return t == TCG_F32 || t == TCG_F16 || t == TCG_BF16; }
@@ -403,19 +433,14 @@ tcg_status tcg_linear_s8_grouped(const void* x, tcg_dtype x_type, const int8_t* 
     if (misaligned(x, size_of(x_type)) || misaligned(B, 16) || misaligned(C, size_of(c_type)) ||
         misaligned(scale_b, 4) || misaligned(bias, 4))
         return TCG_ERR_ALIGN;
-    if (!offsets && groups == 1 && M <= kOwnRows && !misaligned(x, 16)) {
-        int dev, sms;
-        if ((s = host::device(&dev, &sms)) != TCG_SUCCESS) return s;
-        RowsCall c = s8_call(nullptr, B, C, c_type, nullptr, 1, M, N, K, nullptr, scale_b, bias, 0);
-        c.x = x;
-        c.x_type = x_type;
-        RowsPlan plan;
-        if (owns_rows(c, sms, &plan))
-            return launch<RowsTraits<kKindI8, false, false, 1, 16, true>>(c, plan.split, plan.chunk, dev, sms,
-                                                                          static_cast<cudaStream_t>(stream));
+    if (!offsets && groups == 1 && few_rows(M, N, K) && !misaligned(x, 16)) {
+        const FewParams p{x, B, C, scale_b, bias, N, K, c_type};
+        const cudaStream_t st = static_cast<cudaStream_t>(stream);
+        if (x_type == TCG_F32) return run_few<float>(p, M, st);
+        if (x_type == TCG_F16) return run_few<__half>(p, M, st);
+        return run_few<__nv_bfloat16>(p, M, st);
     }
-    if (!workspace) return TCG_ERR_ARG;
-    if (workspace_bytes < tcg_linear_s8_workspace_size(M, K)) return TCG_ERR_WORKSPACE;
+    if (!workspace || workspace_bytes < tcg_linear_s8_workspace_size(M, K)) return TCG_ERR_WORKSPACE;
     if (misaligned(workspace, 256)) return TCG_ERR_ALIGN;
     int8_t* codes = static_cast<int8_t*>(workspace);
     float* scale = reinterpret_cast<float*>(codes + round256(static_cast<size_t>(M) * K));

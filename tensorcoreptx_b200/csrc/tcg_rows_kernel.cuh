@@ -48,14 +48,11 @@
 #include <cuda_fp16.h>
 
 #include "tcg_ptx.cuh"
-#include "tcg_rowquant.cuh"
 #include "tcg_wait.cuh"
 
 namespace tcg {
 
 constexpr int kRowsMaxGroups = 1024;
-constexpr int kOwnRows = 3;    // kOwn: most rows that a product quantises itself,
-constexpr int kOwnBlocks = 32; // and most k-blocks of them that a CTA keeps
 
 constexpr int kOutF32 = 0, kOutF16 = 1, kOutBF16 = 2;  // tcg_dtype
 
@@ -63,8 +60,6 @@ struct RowsParams {
     void* out;
     const int* offsets;       // groups + 1 row bounds on the device; null: groups of `rows_per_group`
     const float* scale_q;     // int8: one per row
-    const void* x;            // kOwn: the rows to quantise
-    int x_type, own_blocks;   // kOwn: their type; k-blocks of them that a CTA keeps
     const float* scale_p;     // int8: one per group and feature
     const float* bias_p;      // int8: one per group and feature, or null
     unsigned long long timeout_ns;
@@ -85,12 +80,11 @@ struct RowsParams {
     uint32_t idesc;           // instruction descriptor without N
 };
 
-template <int kKind_, bool kPMn_, bool kQMn_, int kSub_, int kBQ_, bool kOwn_ = false>
+template <int kKind_, bool kPMn_, bool kQMn_, int kSub_, int kBQ_>
 struct RowsTraits {
     static constexpr int kKind = kKind_;
     static constexpr bool kPMn = kPMn_, kQMn = kQMn_;
     static constexpr int kSub = kSub_, kBQ = kBQ_;
-    static constexpr bool kOwn = kOwn_;                 // the rows are quantised here (own_absmax, own_codes)
     static constexpr bool kWeight = kQMn;               // weight form: the sum runs over a group's rows
     static constexpr int kElem = kKind == kKindF16 ? 2 : 1;
     static constexpr int kBK = 128 / kElem;             // length of the sum per ring stage
@@ -99,7 +93,7 @@ struct RowsTraits {
     static constexpr int kSubBytes = 128 * kBK * kElem; // one 128-feature block of a stage
     static constexpr int kPBytes = kSub * kSubBytes;
     static constexpr int kQBytes = kBQ * kBK * kElem;
-    static constexpr int kStageBytes = kPBytes + (kOwn ? 0 : kQBytes);
+    static constexpr int kStageBytes = kPBytes + kQBytes;
     static constexpr int kAtomBytes = 128 * kBK;        // MN-major: 64 elements of kBK rows
     static constexpr int kQBox = kBQ < 64 ? kBQ : 64;   // rows (weight form: columns) per box of the q operand
     static constexpr int kQBoxBytes = kQBox * kBK * kElem;
@@ -120,14 +114,13 @@ struct RowsTraits {
     static_assert(!kQMn || kKind == kKindF16, "weight form: 16-bit operands");
     static_assert(!kPMn || kKind == kKindF16, "MN-major features: 16-bit operands");
     static_assert(!kQMn || kBQ % 64 == 0, "whole 64-column atoms");
-    static_assert(!kOwn || (kKind == kKindI8 && kSub == 1 && kBQ == 16), "rows quantised here: few, int8");
     static_assert(8 * (2 * kMaxStages + 6 + 2 * kRing) + 8 + 4 * kRing + 16 <= kBarBytes - 16, "barrier area");
     static_assert((kTmemCols & (kTmemCols - 1)) == 0 && kTmemCols <= 512, "TMEM allocation");
     // dynamic shared memory of a launch with a table of `groups` groups
-    static constexpr int smem_bytes(int stages, int split, int groups, int own_blocks)
+    static constexpr int smem_bytes(int stages, int split, int groups)
     {
-        return 1024 + stages * kStageBytes + kOutArea + own_blocks * kQBytes + (split > 1 ? kRedBytes : 0) +
-               kScaleBytes + kBarBytes + 8 * (groups + 3);
+        return 1024 + stages * kStageBytes + kOutArea + (split > 1 ? kRedBytes : 0) + kScaleBytes + kBarBytes +
+               8 * (groups + 3);
     }
 };
 
@@ -393,69 +386,6 @@ __device__ __forceinline__ void store_block32(const float (&x)[32], const OutBlo
     }
 }
 
-// kOwn: a product of up to kOwnRows rows quantises them itself -- every CTA the
-// whole rows' absmax, then the codes of its own k-blocks into shared memory, in
-// the K-major 128-byte-swizzled layout the MMA reads (one block of 16 rows x 128
-// bytes per k-block), while the weights are on their way.  The codes and scales
-// are those of quantize_rows_kernel.  Saves a launch and the trip of the codes
-// through memory, and costs every CTA the rows' absmax: 4096 x 4096 with one row
-// 7.9 us (two kernels 8.9), two 8.3, three 8.9, four 9.3 -- hence at most three.
-// By the epilogue's 256 threads (t), the absmax before the kernel's first block
-// barrier, whose cost its loads hide; part is 8 words of scratch per row.  (What
-// is left in rows >= rows and past K is never used: those columns are not
-// stored, and the weights are zero past K.)
-template <class T>
-__device__ __forceinline__ void own_absmax(const T* x, int rows, int k, uint32_t* part, int t)
-{
-    const int nv = k / RowVec<T>::kN;
-    uint32_t m[kOwnRows];
-#pragma unroll
-    for (int r = 0; r < kOwnRows; ++r) {
-        m[r] = 0u;
-        if (r < rows) {
-            const uint4* xv = reinterpret_cast<const uint4*>(x + static_cast<long long>(r) * k);
-#pragma unroll 4
-            for (int i = t; i < nv; i += 256) m[r] = row_absmax<T>(xv[i], m[r]);
-        }
-    }
-#pragma unroll
-    for (int r = 0; r < kOwnRows; ++r) {
-        if (r < rows) m[r] = __reduce_max_sync(0xffffffffu, __float_as_uint(row_magnitude<T>(m[r])));
-        if ((t & 31) == 0) part[r * 8 + (t >> 5)] = m[r];
-    }
-}
-
-// After the barrier: scale[r] and its inverse by one thread a row, then the
-// codes of k-blocks [kb0, kb1) of all rows together.
-template <class T>
-__device__ __forceinline__ void own_codes(const T* x, int rows, int k, int kb0, int kb1, uint8_t* own, float* scale,
-                                          const uint32_t* part, int t)
-{
-    constexpr int kN = RowVec<T>::kN;
-    float* inv = scale + kOwnRows;
-    if (t < rows) {
-        uint32_t top = 0u;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = max(top, part[t * 8 + i]);
-        const float absmax = __uint_as_float(top);
-        scale[t] = __fdiv_rn(absmax, 127.f);
-        inv[t] = quant_inv(absmax, 127.f);
-    }
-    asm volatile("bar.sync 1, 256;" ::: "memory");
-    const int v0 = kb0 * (128 / kN), n = min(kb1 * (128 / kN), k / kN) - v0;
-    for (int i = t; i < rows * n; i += 256) {
-        const int r = i < n ? 0 : (i < 2 * n ? 1 : 2);
-        const int v = i - r * n;
-        const uint4 xv = *reinterpret_cast<const uint4*>(x + static_cast<long long>(r) * k + (v0 + v) * kN);
-        const bool plain = scale[r] > 1e-32f && scale[r] < 2e36f;
-        const int byte = v * kN;  // of this CTA's slice of the row
-        const int chunk = ((byte >> 4) & 7) ^ r;
-        row_codes<T>(xv, inv[r], plain,
-                     reinterpret_cast<int8_t*>(own + (byte >> 7) * 2048 + r * 128 + (chunk << 4) + (byte & 15)));
-    }
-    fence_proxy_async_smem();
-}
-
 // Split sums.  Columns c .. c + n - 1 of this CTA's part (one lane = feature
 // f) to the CTAs that finish them: CTA d finishes columns d * kBQ / S onwards.
 // There the parts lie as [source rank][group of V columns][feature][V], V = 4
@@ -544,8 +474,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
     const int S = C::kSub == 1 ? 1 << p.split_log2 : 1;
     const int stages = p.stages;
     uint8_t* out_area = C::kSub == 2 ? smem + stages * C::kStageBytes : smem;
-    uint8_t* own_area = smem + stages * C::kStageBytes + C::kOutArea;  // 1024-byte aligned
-    uint32_t* red = reinterpret_cast<uint32_t*>(own_area + (C::kOwn ? p.own_blocks * C::kQBytes : 0));
+    uint32_t* red = reinterpret_cast<uint32_t*>(smem + stages * C::kStageBytes + C::kOutArea);
     float* scales = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(red) + (S > 1 ? C::kRedBytes : 0));
     uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(scales) + C::kScaleBytes);
     uint64_t* empty = full + C::kMaxStages;
@@ -579,7 +508,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
             mbar_init(smem_u32(clcbar), 1);
             *abort_flag = 0u;
         } else if (lane >= 24 && lane < 24 + C::kRing) {
-            mbar_init(smem_u32(&qfull[lane - 24]), C::kOwn ? C::kEpiWarps : 1);
+            mbar_init(smem_u32(&qfull[lane - 24]), 1);
             mbar_init(smem_u32(&qempty[lane - 24]), 1 + C::kEpiWarps);
         } else if (lane == 19) {
             tma_prefetch_desc(&tmP);
@@ -600,16 +529,6 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
     if (!p.early) grid_dependency_wait();
     grid_launch_dependents();
     if (p.offsets && warp == 2) rows_table(p, C::kBQ, bound, cum);
-    uint32_t* own_part = reinterpret_cast<uint32_t*>(scales + 64);
-    if (C::kOwn && warp >= 2) {
-        const int t = static_cast<int>(threadIdx.x) - 64;
-        if (p.x_type == kOutF32)
-            own_absmax(static_cast<const float*>(p.x), p.rows, p.R, own_part, t);
-        else if (p.x_type == kOutF16)
-            own_absmax(static_cast<const __half*>(p.x), p.rows, p.R, own_part, t);
-        else
-            own_absmax(static_cast<const __nv_bfloat16*>(p.x), p.rows, p.R, own_part, t);
-    }
     tc_fence_before();
     __syncthreads();
     if (S > 1) cluster_arrive();  // every CTA of the cluster runs before any writes into another (push_part)
@@ -684,7 +603,6 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
         };
         const auto load_q = [&](const RowsItem& w, int kb, int st, int boxes) {
             const uint32_t dst = ring + st * C::kStageBytes + C::kPBytes, fb = smem_u32(&full[st]);
-            if constexpr (C::kOwn) return;
             if constexpr (C::kQMn) {
                 if (p.q_whole)
                     tma_load_4d(dst, &tmQ, fb, 0, w.row0 + kb * C::kBK, w.q0 / 64, 0);
@@ -737,7 +655,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
             const int boxes = (w.cnt + C::kQBox - 1) / C::kQBox;
             const int p_bytes = C::kPMn && !p.p_whole ? blocks * C::kSubBytes : C::kPBytes;
             const int q_bytes = C::kQMn && p.q_whole ? C::kQBytes : boxes * C::kQBoxBytes;
-            const uint32_t tx = static_cast<uint32_t>(p_bytes + (C::kOwn ? 0 : q_bytes));
+            const uint32_t tx = static_cast<uint32_t>(p_bytes + q_bytes);
             int kb = kb0;
             if (!waited) {
                 // the first ring-full: features now, rows once the kernel before has finished
@@ -807,7 +725,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
         bool aborted = false;
         const uint64_t pdesc = C::kPMn ? smem_desc_sw128(ring, C::kAtomBytes, 1024) : smem_desc_sw128(ring, 16, 1024);
         const uint64_t qdesc = C::kQMn ? smem_desc_sw128(ring + C::kPBytes, C::kAtomBytes, 1024)
-                                       : smem_desc_sw128(C::kOwn ? smem_u32(own_area) : ring + C::kPBytes, 16, 1024);
+                                       : smem_desc_sw128(ring + C::kPBytes, 16, 1024);
         for (int item = next_item(-1); item >= 0 && !aborted; item = next_item(item)) {
             const RowsItem w = uniform(tile_of(item));
             int kb0, kb1;
@@ -851,8 +769,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
 #pragma unroll
                     for (int k = 0; k < C::kBK / C::kUmmaK; ++k) {
                         if (k >= ksteps) break;
-                        const uint64_t qat = C::kOwn ? static_cast<uint64_t>((kb - kb0) * (C::kQBytes / 16)) : at;
-                        const uint64_t qd = qdesc + qat + k * (C::kQMn ? C::kUmmaK * 8 : 2);
+                        const uint64_t qd = qdesc + at + k * (C::kQMn ? C::kUmmaK * 8 : 2);
                         const uint64_t pd = pdesc + at + k * (C::kPMn ? C::kUmmaK * 8 : 2);
                         const uint32_t sum = !fresh || k > 0 ? 1u : 0u;
                         if (mask & 1) umma<C::kKind>(d, pd, qd, idesc, sum);
@@ -937,9 +854,6 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                 }
                 complete(1);
             } else {
-                if (C::kOwn && !wait_bounded_warp(smem_u32(&qfull[0]), 0, abort_flag, p.timeout_ns,
-                                                  (blockIdx.x << 8) | 0x70u))
-                    break;  // the rows' codes are in place
                 // Chunks of the sum into two accumulators in turn: the epilogue
                 // takes one to its registers while the other fills.
                 int part = 0;  // k-blocks of the chunk so far
@@ -977,23 +891,6 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
         uint32_t acc_phase = 0;
         bool lost = false;
         if (p.early) grid_dependency_wait();  // the rows' scales, and the output's last readers
-        if constexpr (C::kOwn) {
-            if (total > 0) {
-                const RowsItem w = tile_of(0);
-                int kb0, kb1;
-                share(w, kb0, kb1);
-                const int t = static_cast<int>(threadIdx.x) - 64;
-                if (p.x_type == kOutF32)
-                    own_codes(static_cast<const float*>(p.x), w.cnt, p.R, kb0, kb1, own_area, scales, own_part, t);
-                else if (p.x_type == kOutF16)
-                    own_codes(static_cast<const __half*>(p.x), w.cnt, p.R, kb0, kb1, own_area, scales, own_part, t);
-                else
-                    own_codes(static_cast<const __nv_bfloat16*>(p.x), w.cnt, p.R, kb0, kb1, own_area, scales, own_part, t);
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&qfull[0]));
-                group_sync(2 + group);  // (group 0 has written the scales and reads them)
-            }
-        }
         if (S > 1) cluster_wait();
         for (int item = next_item(-1); item >= 0 && !lost; item = next_item(item)) {
             const RowsItem w = tile_of(item);
@@ -1026,10 +923,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
             const auto rows_scales = [&](int c) {
                 if (C::kKind == kKindI8) {  // the rows' scales, for every lane to read
                     __syncwarp();
-                    const float own = C::kOwn && c + lane < w.cnt ? scales[c + lane] : 0.f;
-                    __syncwarp();
-                    warp_scales[lane] =
-                        C::kOwn ? own : (!w.zero && c + lane < w.cnt ? p.scale_q[w.row0 + c + lane] : 0.f);
+                    warp_scales[lane] = !w.zero && c + lane < w.cnt ? p.scale_q[w.row0 + c + lane] : 0.f;
                     __syncwarp();
                 }
             };
@@ -1202,7 +1096,6 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
         RowsItem w;
         float sp = 0.f, bias = 0.f;
         const int per = C::kBQ >> p.split_log2;
-        const int own0 = C::kOwn ? rank * per : 0;  // kOwn: the scales of all rows are there
         const int t = static_cast<int>(threadIdx.x);
         if (work) {
             w = tile_of(0);
@@ -1213,7 +1106,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                     if (p.bias_p) bias = p.bias_p[at];
                 }
                 if (p.early) grid_dependency_wait();
-                if (!C::kOwn && t < per)
+                if (t < per)
                     scales[t] = rank * per + t < w.cnt && !w.zero ? p.scale_q[w.row0 + rank * per + t] : 0.f;
             }
         }
@@ -1221,11 +1114,11 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
         cluster_sync_all();            // every part has arrived
         if (work && t < 256) {
             if (p.out_type == kOutF32)
-                finish<C, float>(p, w, red, scales + own0, rank, t, sp, bias);
+                finish<C, float>(p, w, red, scales, rank, t, sp, bias);
             else if (p.out_type == kOutF16)
-                finish<C, __half>(p, w, red, scales + own0, rank, t, sp, bias);
+                finish<C, __half>(p, w, red, scales, rank, t, sp, bias);
             else
-                finish<C, __nv_bfloat16>(p, w, red, scales + own0, rank, t, sp, bias);
+                finish<C, __nv_bfloat16>(p, w, red, scales, rank, t, sp, bias);
         }
     }
     tc_fence_after();

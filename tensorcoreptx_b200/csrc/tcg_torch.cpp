@@ -186,17 +186,22 @@ Tensor linear_int8(const Tensor& x, const Tensor& BT, const OptTensor& offsets, 
     int zero_rest = 0;
     Tensor C = offsets ? grouped_out(out, x, N, x.scalar_type(), &zero_rest) : like_rows(x, N, x.scalar_type());
     if (C.numel() == 0) return C;
-    const size_t need = tcg_linear_s8_workspace_size(M, static_cast<int>(K));
-    Tensor ws = at::empty({static_cast<int64_t>(need)}, x.options().dtype(at::kByte));
     const On on(x);
-    check_status("tcg_linear_s8_grouped",
-                 tcg_linear_s8_grouped(x.const_data_ptr(), type_of(x.scalar_type()),
-                                       static_cast<const int8_t*>(BT.const_data_ptr()), C.mutable_data_ptr(),
-                                       type_of(x.scalar_type()), offsets ? offsets_ptr(*offsets) : nullptr, groups, M,
-                                       narrow(N, "N"), narrow(K, "K"),
-                                       static_cast<const float*>(scale_b.const_data_ptr()),
-                                       bias ? static_cast<const float*>(bias->const_data_ptr()) : nullptr, zero_rest,
-                                       ws.mutable_data_ptr(), need, on.stream));
+    const auto call = [&](void* workspace, size_t bytes) {
+        return tcg_linear_s8_grouped(
+            x.const_data_ptr(), type_of(x.scalar_type()), static_cast<const int8_t*>(BT.const_data_ptr()),
+            C.mutable_data_ptr(), type_of(x.scalar_type()), offsets ? offsets_ptr(*offsets) : nullptr, groups, M,
+            narrow(N, "N"), narrow(K, "K"), static_cast<const float*>(scale_b.const_data_ptr()),
+            bias ? static_cast<const float*>(bias->const_data_ptr()) : nullptr, zero_rest, workspace, bytes, on.stream);
+    };
+    // few rows usually need no workspace; the call says so before it launches anything
+    tcg_status s = offsets || M > 4 ? TCG_ERR_WORKSPACE : call(nullptr, 0);
+    if (s == TCG_ERR_WORKSPACE) {
+        const size_t need = tcg_linear_s8_workspace_size(M, static_cast<int>(K));
+        Tensor ws = at::empty({static_cast<int64_t>(need)}, x.options().dtype(at::kByte));
+        s = call(ws.mutable_data_ptr(), need);
+    }
+    check_status("tcg_linear_s8_grouped", s);
     return C;
 }
 

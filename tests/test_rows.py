@@ -75,7 +75,7 @@ def test_linear_int8_refusals():
     assert L().tcg_linear_s8_workspace_size(1 << 20, 1 << 14) == (1 << 34) + (1 << 22)
     ok = [16, 1, 16, 16, 1, 5, 4, 16, 16, None, 256, need, None]  # more rows than a product quantises itself
     for i, v, st in ((1, 3, ARG), (4, -1, ARG), (0, None, ARG), (2, None, ARG), (3, None, ARG), (8, None, ARG),
-                     (10, None, ARG), (11, need - 1, WORKSPACE), (10, 128, ALIGN), (0, 17, ALIGN), (2, 24, ALIGN),
+                     (10, None, WORKSPACE), (11, need - 1, WORKSPACE), (10, 128, ALIGN), (0, 17, ALIGN), (2, 24, ALIGN),
                      (7, 8, SHAPE), (5, -1, SHAPE)):
         args = list(ok)
         args[i] = v
