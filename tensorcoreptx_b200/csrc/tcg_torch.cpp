@@ -255,12 +255,15 @@ struct LinearFunction : public torch::autograd::Function<LinearFunction> {
             at::NoGradGuard no_grad;
             const auto saved = ctx->get_saved_variables();
             const Tensor &kept = saved[0], &scales = saved[1], &W = saved[2], &offsets = saved[3];
-            const Tensor dy = grads[0].contiguous();
-            if (W.defined()) {
+            Tensor dy = grads[0].contiguous();
+            // (a slice of a larger gradient may start anywhere)
+            if (reinterpret_cast<uintptr_t>(dy.const_data_ptr()) % 16 != 0) dy = dy.clone();
+            // inputs that this pass asks for: x is the function's first, W its second
+            if (W.defined() && ctx->needs_input_grad(0)) {
                 out[0] = like_rows(dy, W.size(-1), dy.scalar_type());
                 product(dy, W, offsets, false, out[0], 1);
             }
-            if (kept.defined())
+            if (kept.defined() && ctx->needs_input_grad(1))
                 out[1] = weight_gradient(dy, scales.defined() ? dequantize(kept, scales, dy.scalar_type()) : kept,
                                          offsets);
         }

@@ -597,6 +597,34 @@ def test_linear_gradient_of_an_expanded_output_and_partial_needs():
     assert not T().linear(x.detach(), W.detach()).requires_grad
 
 
+@pytest.mark.parametrize("save", ["input", "int8"])
+def test_linear_gradient_that_starts_off_a_16_byte_boundary(save):
+    """The output's gradient as a slice of a concatenation's, at an odd element."""
+    g = gen(26)
+    x, W = randn(g, 33, 64, dtype=F16).requires_grad_(True), randn(g, 24, 64, dtype=F16).requires_grad_(True)
+    dy = randn(g, 33, 24, dtype=F16)
+    want = torch.autograd.grad(T().linear(x, W, save=save), (x, W), dy)
+    y = T().linear(x, W, save=save)
+    all_of = torch.cat([torch.zeros(3, dtype=F16, device=DEV), y.flatten()])
+    got = torch.autograd.grad(all_of, (x, W), torch.cat([torch.ones(3, dtype=F16, device=DEV), dy.flatten()]))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_linear_computes_only_the_gradients_that_a_pass_asks_for():
+    g = gen(27)
+    x, W = randn(g, 64, 64, dtype=BF16).requires_grad_(True), randn(g, 2048, 64, dtype=BF16).requires_grad_(True)
+    dy = randn(g, 64, 2048, dtype=BF16)
+    y = T().linear(x, W)
+    both = torch.autograd.grad(y, (x, W), dy, retain_graph=True)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    only_x, = torch.autograd.grad(y, x, dy, retain_graph=True)
+    assert torch.cuda.max_memory_allocated() - before < W.numel() * 2  # no gradient of W was made
+    only_W, = torch.autograd.grad(y, W, dy)
+    assert torch.equal(only_x, both[0]) and torch.equal(only_W, both[1])
+
+
 def test_linear_refuses_a_second_differentiation():
     x, W = torch.randn(8, 64, device=DEV).to(BF16).requires_grad_(True), torch.randn(16, 64, device=DEV).to(BF16)
     W.requires_grad_(True)
