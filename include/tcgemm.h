@@ -147,7 +147,8 @@ tcg_status tcg_dequantize_rows_s8(const int8_t* src, const float* scale, void* d
  * output channel (B is N x K, "BT"):
  *   C[m][n] = (float)(sum_k A[m][k] B[n][k]) * scale_a[m] * scale_b[n] + bias[n]
  * rounded once to c_type.  scale_a: batches x M floats, scale_b and bias (or
- * NULL): batches x N floats, on the device.  K % 16 == 0, A and B 16-byte
+ * NULL): batches x N floats, on the device.  K % 16 == 0 and at most 131056 (up
+ * to there the int32 sums are exact whatever the codes), A and B 16-byte
  * aligned, C aligned to its element; M and N arbitrary.
  * tcg_linear_s8 quantises its left operand itself (tcg_quantize_rows_s8) into
  * `workspace` (tcg_linear_s8_workspace_size bytes, 256-byte aligned, not
@@ -169,7 +170,7 @@ tcg_status tcg_linear_s8(const void* x, tcg_dtype x_type, const int8_t* B, void*
  * TCG_MAX_GROUPS), any of the groups empty; they are clamped to be ascending
  * and within 0 .. M.  Rows of C outside every group are set to zero
  * (zero_rest != 0) or left as they are.  NULL offsets: `groups` (at most
- * 65535) groups of M / groups rows each (M % groups == 0).
+ * 65535) groups of M / groups rows each (M % groups == 0).  C overlaps no input.
  * tcg_gemm_16_grouped: A and B fp16 or bf16 (`type`), fp32 sums, C rounded once
  * to c_type; B is groups x N x K (TCG_B_NK) or groups x K x N (TCG_B_KN); K % 8
  * == 0 (and N % 8 == 0 for TCG_B_KN).  The gradient by A is the same product

@@ -318,6 +318,9 @@ bool few_rows(int M, int N, int K)
 bool is_type(tcg_dtype t) { return t == TCG_F32 || t == TCG_F16 || t == TCG_BF16; }
 bool misaligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) % n) != 0; }
 unsigned size_of(tcg_dtype t) { return t == TCG_F32 ? 4u : 2u; }
+// Longest sum of an int8 product: the int32 sums are exact whatever the codes
+// as long as 128 * 128 * K is below 2^31.
+constexpr int kMostK8 = 131056;
 size_t round256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 
 // Checks shared by every form; *done: there is no output.
@@ -362,7 +365,7 @@ tcg_status gemm_s8(const int8_t* A, const int8_t* B, void* C, tcg_dtype c_type, 
                    int early, cudaStream_t st)
 {
     if (!A || !B || !C || !scale_a || !scale_b) return TCG_ERR_ARG;
-    if (K == 0 || K % 16 != 0) return TCG_ERR_SHAPE;
+    if (K == 0 || K % 16 != 0 || K > kMostK8) return TCG_ERR_SHAPE;
     if (misaligned(A, 16) || misaligned(B, 16) || misaligned(C, size_of(c_type)) || misaligned(scale_a, 4) ||
         misaligned(scale_b, 4) || misaligned(bias, 4))
         return TCG_ERR_ALIGN;
@@ -429,7 +432,7 @@ tcg_status tcg_linear_s8_grouped(const void* x, tcg_dtype x_type, const int8_t* 
     if (s != TCG_SUCCESS || done) return s;
     // everything is checked before the first launch
     if (!x || !B || !C || !scale_b) return TCG_ERR_ARG;
-    if (K == 0 || K % 16 != 0) return TCG_ERR_SHAPE;
+    if (K == 0 || K % 16 != 0 || K > kMostK8) return TCG_ERR_SHAPE;
     if (misaligned(x, size_of(x_type)) || misaligned(B, 16) || misaligned(C, size_of(c_type)) ||
         misaligned(scale_b, 4) || misaligned(bias, 4))
         return TCG_ERR_ALIGN;

@@ -90,8 +90,15 @@ Tensor like_rows(const Tensor& x, int64_t last, at::ScalarType type)
 
 int64_t rows_of(const Tensor& x) { return x.size(-1) ? x.numel() / x.size(-1) : 0; }
 
+bool overlap(const Tensor& a, const Tensor& b)
+{
+    const char *pa = static_cast<const char*>(a.const_data_ptr()), *pb = static_cast<const char*>(b.const_data_ptr());
+    return pa < pb + b.nbytes() && pb < pa + a.nbytes();
+}
+
 // The given result, or a new one, whose rows outside the groups become zeros.
-Tensor grouped_out(const OptTensor& out, const Tensor& A, int64_t N, at::ScalarType type, int* zero_rest)
+Tensor grouped_out(const OptTensor& out, const Tensor& A, std::initializer_list<OptTensor> inputs, int64_t N,
+                   at::ScalarType type, int* zero_rest)
 {
     *zero_rest = !out.has_value();
     if (!out) return at::empty({A.size(0), N}, A.options().dtype(type));
@@ -99,6 +106,7 @@ Tensor grouped_out(const OptTensor& out, const Tensor& A, int64_t N, at::ScalarT
                     out->size(1) == N && out->scalar_type() == type,
                 "out must be a contiguous CUDA tensor of shape [", A.size(0), ", ", N, "] and type ", type);
     same_device(A, "out", *out);
+    for (const OptTensor& t : inputs) TORCH_CHECK(!t || !overlap(*out, *t), "out must not overlap the inputs");
     return *out;
 }
 
@@ -184,7 +192,7 @@ Tensor linear_int8(const Tensor& x, const Tensor& BT, const OptTensor& offsets, 
     if (bias) check_floats("bias", *bias, channels, x);
     const int M = narrow(rows_of(x), "the number of rows");
     int zero_rest = 0;
-    Tensor C = offsets ? grouped_out(out, x, N, x.scalar_type(), &zero_rest) : like_rows(x, N, x.scalar_type());
+    Tensor C = offsets ? grouped_out(out, x, {x, BT, offsets, scale_b, bias}, N, x.scalar_type(), &zero_rest) : like_rows(x, N, x.scalar_type());
     if (C.numel() == 0) return C;
     const On on(x);
     const auto call = [&](void* workspace, size_t bytes) {
@@ -219,7 +227,7 @@ Tensor gemm_grouped(const Tensor& A, const Tensor& B, const Tensor& offsets, boo
     same_device(A, "B", B);
     check_offsets(offsets, B.size(0), A);
     int zero_rest;
-    Tensor C = grouped_out(out, A, B.size(nk ? 1 : 2), type, &zero_rest);
+    Tensor C = grouped_out(out, A, {A, B, offsets}, B.size(nk ? 1 : 2), type, &zero_rest);
     product(A, B, offsets, nk, C, zero_rest);
     return C;
 }

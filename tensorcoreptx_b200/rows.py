@@ -12,13 +12,13 @@ grouped by expert, and layers that train through them.
 Like the other entries they check their arguments (``RuntimeError``), return
 new tensors on the inputs' device, run asynchronously on that device's current
 stream, and can be captured into CUDA graphs.  There is no CPU or library
-fallback.  Inputs are contiguous; products need K to be a multiple of 16 (int8)
-or 8 (16 bits); the number of rows is arbitrary.
+fallback.  Inputs are contiguous; products need K to be a multiple of 16 (int8,
+at most 131056, so that the int32 sums are exact) or 8 (16 bits); the number of rows is arbitrary.
 
 ``offsets`` (int32, groups + 1 values on the device) are the ascending row
 bounds of the groups: group e is rows ``offsets[e]`` to ``offsets[e + 1] - 1``,
 any of them empty.  Rows outside every group (a padded batch) give zeros in a
-new result and are left alone in a given one.  Offsets that descend or exceed
+new result and are left alone in a given one (``out``, which overlaps no input).  Offsets that descend or exceed
 the rows are clamped, never followed out of range.
 """
 from __future__ import annotations
@@ -75,7 +75,13 @@ def _check_floats(name: str, t, shape, like):
     _same_device(like, name, t)
 
 
-def _grouped_out(out, A, M: int, N: int, dtype):
+def _overlap(a, b) -> bool:
+    """Whether two contiguous tensors share memory."""
+    return (a.data_ptr() < b.data_ptr() + b.numel() * b.element_size() and
+            b.data_ptr() < a.data_ptr() + a.numel() * a.element_size())
+
+
+def _grouped_out(out, A, inputs, M: int, N: int, dtype):
     """(result, zero_rest): a new result whose rows outside the groups become
     zeros, or the given one, whose rows there stay."""
     if out is None:
@@ -83,6 +89,7 @@ def _grouped_out(out, A, M: int, N: int, dtype):
     if not (out.is_cuda and out.is_contiguous() and out.shape == (M, N) and out.dtype == dtype):
         raise RuntimeError(f"out must be a contiguous CUDA tensor of shape {(M, N)} and type {dtype}")
     _same_device(A, "out", out)
+    _check(not any(_overlap(out, t) for t in inputs if t is not None), "out must not overlap the inputs")
     return out, 0
 
 
@@ -173,7 +180,7 @@ def gemm_int8_grouped(A: torch.Tensor, BT: torch.Tensor, offsets: torch.Tensor, 
     _check_floats("scale_b", scale_b, (E, N), A)
     if bias is not None:
         _check_floats("bias", bias, (E, N), A)
-    C, rest = _grouped_out(out, A, M, N, out_dtype)
+    C, rest = _grouped_out(out, A, (A, BT, offsets, scale_a, scale_b, bias), M, N, out_dtype)
     _call("tcg_gemm_s8_grouped", A, A.data_ptr(), BT.data_ptr(), C.data_ptr(), _TYPES[out_dtype], offsets.data_ptr(),
           E, M, N, K, scale_a.data_ptr(), scale_b.data_ptr(), _ptr(bias), rest)
     return C

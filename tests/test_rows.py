@@ -53,6 +53,7 @@ def test_int8_product_refusals():
     assert f(16, 16, 16, 1, 4, 4, 0, 1, 16, 16, None, None) == SHAPE
     assert f(16, 16, 16, 1, 4, 4, 16, 65536, 16, 16, None, None) == SHAPE
     assert f(16, 16, 16, 1, 1 << 30, 4, 16, 4, 16, 16, None, None) == SHAPE  # 2^32 rows
+    assert f(16, 16, 16, 1, 4, 4, 131072, 1, 16, 16, None, None) == SHAPE  # a sum could pass 2^31
     for i in (0, 1, 2, 8, 9):
         args = [16, 16, 16, 1, 4, 4, 16, 1, 16, 16, None, None]
         args[i] = None
@@ -76,7 +77,7 @@ def test_linear_int8_refusals():
     ok = [16, 1, 16, 16, 1, 5, 4, 16, 16, None, 256, need, None]  # more rows than a product quantises itself
     for i, v, st in ((1, 3, ARG), (4, -1, ARG), (0, None, ARG), (2, None, ARG), (3, None, ARG), (8, None, ARG),
                      (10, None, WORKSPACE), (11, need - 1, WORKSPACE), (10, 128, ALIGN), (0, 17, ALIGN), (2, 24, ALIGN),
-                     (7, 8, SHAPE), (5, -1, SHAPE)):
+                     (7, 8, SHAPE), (7, 131072, SHAPE), (5, -1, SHAPE)):
         args = list(ok)
         args[i] = v
         assert f(*args) == st, (i, v)

@@ -816,3 +816,17 @@ def test_serving_and_training_products_together():
     bound = sx[:, None] * aw.sum(2)[e] + ax.sum(1)[:, None] * sw[e] + K * sx[:, None] * sw[e]
     rel = half_step(BF16)[0]
     assert ((y8.double() - y16.double()).abs() <= bound * (1 + 4 * rel) + 2.1 * rel * y16.double().abs() + 1e-4).all()
+
+
+@pytest.mark.parametrize("op", ["quantize_rows", "dequantize_rows", "gemm_int8_scaled", "linear_int8"])
+def test_opbench_runs(op, capsys):
+    from tensorcoreptx_b200 import opbench
+    opbench.main([op, "--m", "96", "--n", "128", "--k", "256", "--iters", "2", "--warmup", "1"])
+    assert "per call" in capsys.readouterr().out
+
+
+@pytest.mark.parametrize("op", ["gemm_grouped", "gemm_grouped_wgrad", "linear_int8_grouped", "linear_train", "linear_train_int8"])
+def test_opbench_runs_by_groups(op, capsys):
+    from tensorcoreptx_b200 import opbench
+    opbench.main([op, "--m", "96", "--n", "128", "--k", "256", "--groups", "3", "--iters", "2", "--warmup", "1"])
+    assert "per call" in capsys.readouterr().out

@@ -47,6 +47,12 @@ def test_quantize_and_int8_products():
     refuse("scale_b must have shape", T.linear_int8_grouped, z(4, 16), g, o, sb)
     refuse("out must be", T.linear_int8_grouped, z(4, 16), g, o, z(2, 6, dtype=f32), out=z(4, 7))
     refuse("out must be", T.gemm_int8_grouped, a, g, o, sa, z(2, 6, dtype=f32), out=z(4, 6, dtype=f32))
+    x = z(4, 32)
+    refuse("overlap", T.linear_int8_grouped, x.view(-1)[64:].view(4, 16), g[:, :4].contiguous(), o, z(2, 4, dtype=f32),
+           out=x.view(-1)[60:76].view(4, 4))
+    buf = z(4 * 16 + 4 * 6 * 2, dtype=i8)
+    refuse("overlap", T.gemm_int8_grouped, buf[:64].view(4, 16), g, o, sa, z(2, 6, dtype=f32),
+           out=buf[62:110].view(torch.float16).view(4, 6))
 
 
 def test_16_bit_products_and_layers():
@@ -63,6 +69,7 @@ def test_16_bit_products_and_layers():
     refuse("number of groups", T.gemm_grouped, a, z(1025, 8, 16), z(1026, dtype=torch.int32))
     refuse("SHAPE", T.gemm_grouped, z(4, 12), z(2, 8, 12), o)
     refuse("out must be", T.gemm_grouped, a, b, o, out=z(4, 8, dtype=bf))
+    refuse("overlap", T.gemm_grouped, a, z(2, 16, 16), o, out=a)
     refuse("ALIGN", T.gemm_grouped, z(65)[1:].view(4, 16), b, o)
     refuse("dC's type", T.gemm_grouped_wgrad, z(4, 8), z(4, 16, dtype=bf), o)
     refuse("dC's type", T.gemm_grouped_wgrad, z(4, 8), z(4, 16), o, scale_a=z(4, dtype=torch.float32))
