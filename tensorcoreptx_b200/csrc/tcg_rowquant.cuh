@@ -1,6 +1,6 @@
 // tcg_rowquant.cuh -- the arithmetic of absmax quantisation that the quantising
-// kernels (tcg_quant.cuh) and the products that quantise their own rows
-// (tcg_rows_kernel.cuh) share.
+// kernels (tcg_quant.cuh) and the product that quantises its own rows
+// (tcg_fewrows.cuh) share.
 #pragma once
 
 #include <cstdint>

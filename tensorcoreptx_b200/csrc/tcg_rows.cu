@@ -1,6 +1,6 @@
 // tcg_rows.cu -- host side of the row-scaled and grouped products declared in
 // include/tcgemm.h: checks of arguments, choice of the tile, tensor maps and
-// the launch of rows_kernel (tcg_rows_kernel.cuh).
+// the launch of rows_kernel (tcg_rows_kernel.cuh) or few_rows_kernel (tcg_fewrows.cuh).
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -70,11 +70,17 @@ RowsPlan choose_plan(const RowsCall& c, bool weight, int kblock, int sms)
     const double mean = static_cast<double>(c.rows) / c.groups;  // rows per group
     const double kb = weight ? (mean + kblock - 1) / kblock : ceil_div(c.R, kblock);
     const double used = c.groups < c.rows ? c.groups : c.rows;   // groups that can have rows
-    // fp32 results of long 16-bit sums: in chunks of 512, which the tiles of 256
-    // rows have no room for
-    const bool fine = kblock == 64 && c.out_type == kOutF32 && (weight ? c.rows : c.R) > 512;
-    const int chunk = fine ? 8 : 0x7fffffff;
-    RowsPlan best{128, 1, chunk};
+    // fp32 results of 16-bit sums: in chunks, which the tiles of 256 rows have no
+    // room for.  Few rows, where the weights' bytes are the bound, take chunks of
+    // 128 (86.5 us against 85.7 unchunked, 64 rows of 32 groups x 4096 x 2048);
+    // tiles of more rows 256, or 512 in sums beyond 1024, whose error is that of
+    // 256 in a sum of 1024 by an fp32 product's growth with its square root (8
+    // groups, 4096 rows x 1536 x 2048: 41.9 us in chunks of 512, 44.3 in 256,
+    // 55.6 in 128).
+    const bool wide = kblock == 64 && c.out_type == kOutF32;
+    const int length = weight ? c.rows : c.R;
+    const bool fine = wide && length > 256;
+    RowsPlan best{128, 1, 0x7fffffff};
     double least = -1;
     for (int bq = weight ? 128 : 16; bq <= 256; bq *= 2) {
         if (forced && bq != forced && !(weight && forced < 128 && bq == 128)) continue;
@@ -100,7 +106,7 @@ RowsPlan choose_plan(const RowsCall& c, bool weight, int kblock, int sms)
                     std::max(1.0, tiles * split / sms) * kb / split * (bq == 128 ? 0.30 : 0.20);
             if (least < 0 || t < least) {
                 least = t;
-                best = RowsPlan{bq, split, chunk};
+                best = RowsPlan{bq, split, !wide ? 0x7fffffff : bq <= 32 ? 2 : length <= 1024 ? 4 : 8};
             }
         }
     }
@@ -338,7 +344,7 @@ tcg_status check(int M, int N, int K, int groups, const int32_t* offsets, long l
     return TCG_SUCCESS;
 }
 
-// The call that multiplies rows A (codes, or null: x quantised on the way).
+// The call that multiplies rows of codes A.
 RowsCall s8_call(const int8_t* A, const int8_t* B, void* C, tcg_dtype c_type, const int32_t* offsets, int groups, int M,
                  int N, int K, const float* scale_a, const float* scale_b, const float* bias, int zero_rest)
 {

@@ -24,10 +24,11 @@
 //     the weights' bytes bound the product and every SM has to pull on memory.
 //     The CTAs of a cluster (1, 2, 4 or 8) split the sum between them and add
 //     their parts through distributed shared memory, in rank order (the result
-//     does not depend on timing).  fp32 results are summed in chunks of 512: the
-//     tensor cores drop the bits that do not fit when they add to an
-//     accumulator, an error that grows with the length of the chain (2.4e-6 of
-//     the result at K = 2048; 0.6e-6 in chunks, added with one rounding each).
+//     does not depend on timing).  fp32 results are summed in chunks of 128 to
+//     512: the tensor cores drop the bits that do not fit when they add to an
+//     accumulator, an error that grows with the length of the chain (rms of the
+//     result's: 2.5e-6 at K = 2048, an fp32 product 0.8e-6; 0.65e-6 in chunks of
+//     512, 0.34e-6 of 256, 0.19e-6 of 128, added with one rounding each).
 //   kSub = 2: 256 x 256, two M = 128 accumulators that fill the tensor memory,
 //     for many rows, where the tensor cores bound the product.  Persistent CTAs
 //     take every so manieth tile; or, where the number of tiles is known at
