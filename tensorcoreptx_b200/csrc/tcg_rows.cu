@@ -56,10 +56,14 @@ int ceil_div(long long a, long long b) { return static_cast<int>((a + b - 1) / b
 //   split:     5.5 + the same for a share of the k-blocks.  The exchange costs
 //              1.5; a second wave of clusters costs far more than it saves (48
 //              rows x 10240 x 4096 over 2 CTAs 10.9, over 4 in two waves 14.9),
-//              so all clusters have to be resident at once (two CTAs per SM
-//              with tiles of 16 rows: 16 x 10240 x 4096 8.8 against 10.6
-//              unsplit); clusters of eight CTAs fit few of the GPU's processing clusters (16 of them take
-//              two waves), so at most eight of those.
+//              so all clusters have to be resident at once: one CTA per SM, or
+//              two with tiles of 16 rows (16 x 10240 x 4096 8.8 against 10.6
+//              unsplit) and pairs with tiles of up to 64 (160 CTAs: 48 x 10240 x
+//              4096 10.8 against 12.5; 170 x 5000 x 8192 16.4 against 21.7),
+//              while more than 148 CTAs in fours find no room for some (180 x
+//              3000 x 3008 13.9 against 8.7); clusters of eight CTAs fit few of
+//              the GPU's processing clusters (16 of them take two waves), so at
+//              most eight of those.
 //   kSub = 2:  10 + k-blocks x 0.54 (the tensor cores' rate) x whole waves
 // Example: int8 512 x 4096 x 4096 64 rows 13.4 (model 15.1), 128 rows 12.9
 // (13.6), 256 rows 29.1 (27.3); 100 x 4096 x 4096: 32 rows 10.8, 64 rows on two
@@ -96,7 +100,8 @@ RowsPlan choose_plan(const RowsCall& c, bool weight, int kblock, int sms)
         const double tiles = q * ceil_div(c.P, tile_p);
         for (int split = 1; split <= (bq == 256 ? 1 : 8); split *= 2) {
             if (forced_split && bq != 256 && split != forced_split) continue;
-            const bool resident = split == 8 ? tiles <= 8 : tiles * split <= (bq == 16 ? 2 : 1) * sms;
+            const int per_sm = bq == 16 || (bq <= 64 && split == 2) ? 2 : 1;
+            const bool resident = split == 8 ? tiles <= 8 : tiles * split <= per_sm * sms;
             if (split > 1 && !resident && !forced_split) continue;
             double t;
             if (bq == 256)
