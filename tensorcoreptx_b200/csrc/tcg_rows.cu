@@ -46,6 +46,16 @@ struct RowsPlan {
 
 int ceil_div(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
 
+// Tiles of bq rows along the rows; an upper bound of them where the groups'
+// bounds are known to the device only.
+long long most_row_tiles(const RowsCall& c, int bq)
+{
+    if (!c.offsets) return static_cast<long long>(c.groups) * ceil_div(c.rows / c.groups, bq);
+    long long parts = c.groups + (c.zero_rest ? 2 : 0);
+    if (parts > c.rows) parts = c.rows;
+    return (c.rows + parts * (bq - 1)) / bq;
+}
+
 // Tile and split: the least of a time model's estimates, in microseconds.  The
 // model is a start (launch, first loads, last stores) plus the k-blocks that
 // the busiest SM works through, each at a measured rate (B200, 36 shapes of
@@ -98,10 +108,13 @@ RowsPlan choose_plan(const RowsCall& c, bool weight, int kblock, int sms)
         else
             q = std::max(used, static_cast<double>(c.rows) / bq + 0.5 * used);
         const double tiles = q * ceil_div(c.P, tile_p);
+        const double bound = weight ? tiles : static_cast<double>(most_row_tiles(c, bq)) * ceil_div(c.P, tile_p);
         for (int split = 1; split <= (bq == 256 ? 1 : 8); split *= 2) {
             if (forced_split && bq != 256 && split != forced_split) continue;
             const int per_sm = bq == 16 || (bq <= 64 && split == 2) ? 2 : 1;
-            const bool resident = split == 8 ? tiles <= 8 : tiles * split <= per_sm * sms;
+            // (tiles of 128 rows take an SM's shared memory, those of empty CTAs too)
+            const double most = bq == 128 ? std::max(tiles, bound) : tiles;
+            const bool resident = split == 8 ? most <= 8 : most * split <= per_sm * sms;
             if (split > 1 && !resident && !forced_split) continue;
             double t;
             if (bq == 256)
@@ -191,13 +204,7 @@ tcg_status launch(const RowsCall& c, int split, int chunk, int dev, int sms, cud
     const uint32_t fmt = C::kKind == kKindI8 ? 1u : (c.bf16 ? 1u : 0u);
     p.idesc = make_idesc(C::kKind == kKindI8 ? 2u : 1u, fmt, fmt, C::kQMn, 128, 0) | (C::kPMn ? 1u << 15 : 0u);
 
-    // an upper bound of the tiles (the bounds of ragged groups are known to the device only)
-    long long qt = static_cast<long long>(c.groups) * p.qtiles;
-    if (!C::kWeight && c.offsets) {
-        long long parts = c.groups + (c.zero_rest ? 2 : 0);
-        if (parts > c.rows) parts = c.rows;
-        qt = (c.rows + parts * (C::kBQ - 1)) / C::kBQ;
-    }
+    const long long qt = C::kWeight ? static_cast<long long>(c.groups) * p.qtiles : most_row_tiles(c, C::kBQ);
     const long long items = qt * p.ptiles;
     if (items > 0x7fffffffLL / 8 || p.ptiles > 65535) return TCG_ERR_SHAPE;
     // bands about square in elements over the tiles in flight
