@@ -62,7 +62,8 @@ long long most_row_tiles(const RowsCall& c, int bq)
 // 1 to 8192 rows and 1 to 64 groups timed with every tile and split):
 //   kSub = 1:  4.0 + k-blocks x 0.20 (tiles of up to 64 rows: the rate at which
 //              one CTA's loads and MMAs are issued) or x 0.30 (128 rows: bytes
-//              from L2), x tiles per SM
+//              from L2), x tiles per SM, and 1.7 or 2.2 a tile after the first
+//              (its start and its stores, of which the CTAs of an SM hide half)
 //   split:     5.5 + the same for a share of the k-blocks.  The exchange costs
 //              1.5; a second wave of clusters costs far more than it saves (48
 //              rows x 10240 x 4096 over 2 CTAs 10.9, over 4 in two waves 14.9),
@@ -74,7 +75,9 @@ long long most_row_tiles(const RowsCall& c, int bq)
 //              3000 x 3008 13.9 against 8.7); clusters of eight CTAs fit few of
 //              the GPU's processing clusters (16 of them take two waves), so at
 //              most eight of those.
-//   kSub = 2:  10 + k-blocks x 0.54 (the tensor cores' rate) x whole waves
+//   kSub = 2:  10 + k-blocks x 0.54 (the tensor cores' rate) for the first whole
+//              wave, 4.5 + k-blocks x 0.54 for the others, at least 7 (128 KB of
+//              results at the rate at which all SMs write, 14 bytes a cycle each)
 // Example: int8 512 x 4096 x 4096 64 rows 13.4 (model 15.1), 128 rows 12.9
 // (13.6), 256 rows 29.1 (27.3); 100 x 4096 x 4096: 32 rows 10.8, 64 rows on two
 // CTAs 9.0, 128 rows on four 8.5.
@@ -116,12 +119,13 @@ RowsPlan choose_plan(const RowsCall& c, bool weight, int kblock, int sms)
             const double most = bq == 128 ? std::max(tiles, bound) : tiles;
             const bool resident = split == 8 ? most <= 8 : most * split <= per_sm * sms;
             if (split > 1 && !resident && !forced_split) continue;
+            const double per = tiles * split / sms;  // tiles that an SM works through
             double t;
             if (bq == 256)
-                t = 10.0 + std::ceil(tiles / sms) * kb * 0.54;
+                t = 10.0 + kb * 0.54 + (std::ceil(per) - 1) * std::max(7.0, 4.5 + kb * 0.54);
             else
-                t = (split > 1 ? 5.5 : 4.0) +
-                    std::max(1.0, tiles * split / sms) * kb / split * (bq == 128 ? 0.30 : 0.20);
+                t = (split > 1 ? 5.5 : 4.0) + std::max(1.0, per) * kb / split * (bq == 128 ? 0.30 : 0.20) +
+                    (split > 1 ? 0.0 : std::max(0.0, per - 1) * (bq == 128 ? 2.2 : 1.7));
             if (least < 0 || t < least) {
                 least = t;
                 best = RowsPlan{bq, split, !wide ? 0x7fffffff : bq <= 32 ? 2 : length <= 1024 ? 4 : 8};
