@@ -87,6 +87,12 @@ struct RowsTraits {
     static constexpr bool kPMn = kPMn_, kQMn = kQMn_;
     static constexpr int kSub = kSub_, kBQ = kBQ_;
     static constexpr bool kWeight = kQMn;               // weight form: the sum runs over a group's rows
+    // kSub = 2: each group of epilogue warps takes one block, whole, so that its
+    // reads of the accumulator overlap the other's stores.  Pays where stores are
+    // most of a tile, in the gradients (16 groups, 300 rows x 2048 x 2048 59.5 ->
+    // 49.2 us, 16384 x 4096 x 2048 224 -> 217); both groups on each block free it
+    // sooner, which the rows form prefers (int8 8192 x 4096 x 512 58 against 66).
+    static constexpr bool kOwnBlock = kWeight && kSub_ == 2;
     static constexpr int kElem = kKind == kKindF16 ? 2 : 1;
     static constexpr int kBK = 128 / kElem;             // length of the sum per ring stage
     static constexpr int kUmmaK = 32 / kElem;
@@ -503,7 +509,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
             mbar_init(smem_u32(&empty[lane]), 1);
         } else if (lane >= 16 && lane < 18) {
             mbar_init(smem_u32(&tfull[lane - 16]), 1);
-            mbar_init(smem_u32(&tempty[lane - 16]), C::kEpiWarps);
+            mbar_init(smem_u32(&tempty[lane - 16]), C::kOwnBlock ? C::kEpiWarps / 2 : C::kEpiWarps);
         } else if (lane == 18) {
             mbar_init(smem_u32(drain), 1);
             mbar_init(smem_u32(clcbar), 1);
@@ -886,7 +892,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
     } else if (warp >= 2 && warp < 2 + C::kEpiWarps) {
         // ---------------------------------------------------- epilogue ----
         const int quarter = warp & 3;
-        const int group = (warp - 2) >> 2;  // the two groups of four warps take 32 columns in turn
+        const int group = (warp - 2) >> 2;  // two groups of four warps: 32 columns each in turn, or a block each
         float* warp_scales = scales + (warp - 2) * 32;
         uint32_t* stage_out = reinterpret_cast<uint32_t*>(out_area + group * C::kOutBytes);
         uint32_t acc_phase = 0;
@@ -1005,68 +1011,85 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                     results(sum[i], x);
                     store(x, block_of(0, c));
                 }
-            } else if (empty_sum) {
-                // rows outside the groups, a group without rows: zeros
-                const float x[32] = {};
-                for (int h = 0; h < C::kSub; ++h)
-                    for (int c = 32 * group; c < w.cnt; c += 64) {
-                        const OutBlock o = block_of(h, c);
-                        if (o.features > 0) store(x, o);
+            } else {
+                // In two parts: blocks 0 and 1, of which this group takes every
+                // other 32 columns; kOwnBlock: the halves of its block.
+                const auto block = [&](int part) { return C::kOwnBlock ? group : part; };
+                const auto column = [&](int part, int i) {
+                    return C::kOwnBlock ? 128 * part + 32 * i : 32 * group + 64 * i;
+                };
+                const auto arrived = [&](int part) {
+                    if (C::kOwnBlock && part == 1) return;
+                    await(block(part), acc_phase);
+                    channel(block(part));
+                };
+                const auto done = [&](int part) {
+                    if (!C::kOwnBlock || part == 1) release(block(part));
+                };
+                if (empty_sum) {
+                    // rows outside the groups, a group without rows: zeros
+                    const float x[32] = {};
+#pragma unroll 1
+                    for (int k = 0; k < 8; ++k) {
+                        const int c = column(k / 4, k % 4);
+                        const OutBlock o = block_of(block(k / 4), c);
+                        if (c < w.cnt && o.features > 0) store(x, o);
                     }
-            } else if (p.out_type != kOutF32 && p.aligned_out) {
-                // Both blocks into registers (128 words a thread) before any
-                // store: the accumulators are free for the next tile after
-                // about 3000 cycles instead of the 11000 that the stores of
-                // all SMs at once take.
-                uint32_t held[2][4][16];
+                } else if (p.out_type != kOutF32 && p.aligned_out) {
+                    // Both parts into registers (128 words a thread) before any
+                    // store: the accumulators are free for the next tile after
+                    // about 3000 cycles instead of the 11000 that the stores of
+                    // all SMs at once take.
+                    uint32_t held[2][4][16];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    if (lost) break;
-                    await(h, acc_phase);
-                    channel(h);
+                    for (int part = 0; part < 2; ++part) {
+                        if (lost) break;
+                        arrived(part);
+                        if (lost) break;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int c = column(part, i);
+                            if (c < w.cnt) {
+                                uint32_t v[32];
+                                float x[32];
+                                load(block(part) * C::kBQ + c, v);
+                                rows_scales(c);
+                                tmem_ld_wait();
+                                results(v, x);
+                                pack_block(x, p.out_type == kOutBF16, held[part][i]);
+                            }
+                        }
+                        done(part);
+                    }
                     if (lost) break;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int c = 32 * group + 64 * i;
-                        if (c < w.cnt) {
+                    for (int part = 0; part < 2; ++part)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int c = column(part, i);
+                            const OutBlock o = block_of(block(part), c);
+                            if (c < w.cnt && o.features > 0)
+                                store_block16(held[part][i], o, stage_out, quarter, lane, 2 + group);
+                        }
+                } else {
+                    for (int part = 0; part < 2; ++part) {
+                        arrived(part);
+                        if (lost) break;
+#pragma unroll 1
+                        for (int i = 0; i < 4; ++i) {
+                            const int c = column(part, i);
+                            const OutBlock o = block_of(block(part), c);
+                            if (c >= w.cnt || o.features <= 0) break;  // (uniform) the tile's end, the last tile's second block
                             uint32_t v[32];
                             float x[32];
-                            load(h * C::kBQ + c, v);
+                            load(block(part) * C::kBQ + c, v);
                             rows_scales(c);
                             tmem_ld_wait();
                             results(v, x);
-                            pack_block(x, p.out_type == kOutBF16, held[h][i]);
+                            store(x, o);
                         }
+                        done(part);
                     }
-                    release(h);
-                }
-                if (lost) break;
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int c = 32 * group + 64 * i;
-                        const OutBlock o = block_of(h, c);
-                        if (c < w.cnt && o.features > 0) store_block16(held[h][i], o, stage_out, quarter, lane, 2 + group);
-                    }
-            } else {
-                for (int h = 0; h < C::kSub; ++h) {
-                    await(h, acc_phase);
-                    channel(h);
-                    if (lost) break;
-#pragma unroll 1
-                    for (int c = 32 * group; c < w.cnt; c += 64) {
-                        const OutBlock o = block_of(h, c);
-                        if (o.features <= 0) break;  // (uniform) the second half of the last tile along P
-                        uint32_t v[32];
-                        float x[32];
-                        load(h * C::kBQ + c, v);
-                        rows_scales(c);
-                        tmem_ld_wait();
-                        results(v, x);
-                        store(x, o);
-                    }
-                    release(h);
                 }
             }
             if (!empty_sum) acc_phase ^= 1u;
