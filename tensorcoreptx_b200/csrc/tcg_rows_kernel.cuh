@@ -109,7 +109,7 @@ struct RowsTraits {
     static constexpr int kPerSm = kSub == 1 ? 2 : 1;  // CTAs per SM that registers are kept for
     // kSub = 1 with fp32 sums: two accumulators that take chunks of the sum in turn
     static constexpr bool kChunks = kSub == 1 && kKind == kKindF16;
-    static constexpr int kTmemCols = kChunks ? 2 * kBQ : (kSub * kBQ < 32 ? 32 : kSub * kBQ);
+    static constexpr int kTmemCols = kChunks ? (kBQ < 32 ? 64 : 2 * kBQ) : (kSub * kBQ < 32 ? 32 : kSub * kBQ);
     static constexpr int kRedBytes = kBQ * 512;         // split: 128 x kBQ partial sums
     static constexpr int kMaxStages = 12;
     static constexpr int kRing = 4;                     // kSub = 2: items on their way to the other roles
@@ -123,6 +123,8 @@ struct RowsTraits {
     static_assert(!kQMn || kBQ % 64 == 0, "whole 64-column atoms");
     static_assert(8 * (2 * kMaxStages + 6 + 2 * kRing) + 8 + 4 * kRing + 16 <= kBarBytes - 16, "barrier area");
     static_assert((kTmemCols & (kTmemCols - 1)) == 0 && kTmemCols <= 512, "TMEM allocation");
+    // the epilogue reads 32 columns at a time, from the start of the last accumulator too
+    static_assert((kChunks || kSub == 2 ? kBQ : 0) + (kBQ < 32 ? 32 : kBQ) <= kTmemCols, "reads inside the allocation");
     // dynamic shared memory of a launch with a table of `groups` groups
     static constexpr int smem_bytes(int stages, int split, int groups)
     {
