@@ -901,7 +901,15 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
         bool lost = false;
         if (p.early) grid_dependency_wait();  // the rows' scales, and the output's last readers
         if (S > 1) cluster_wait();
-        for (int item = next_item(-1); item >= 0 && !lost; item = next_item(item)) {
+        // Dynamic: each warp waits for the item on its own, and on the abort path
+        // one may give up where its neighbours still see the item arrive; the
+        // group takes an item only if all four have it.
+        const auto group_item = [&](int item) {
+            item = next_item(item);
+            if (dynamic && !named_barrier_and(2 + group, 128, item >= 0)) item = -1;
+            return item;
+        };
+        for (int item = group_item(-1); item >= 0 && !lost; item = group_item(item)) {
             const RowsItem w = tile_of(item);
             int kb0, kb1;
             share(w, kb0, kb1);
