@@ -151,7 +151,9 @@ __device__ __forceinline__ void clc_try_cancel(uint32_t resp, uint32_t bar)
 }
 
 // Read a response: true and the x index of the first CTA of the cancelled
-// cluster, or false when no cluster was left to cancel.
+// cluster, or false when no cluster was left to cancel.  The next request's
+// response is written through the asynchronous proxy; the fence orders that
+// behind these loads.
 __device__ __forceinline__ bool clc_query(uint32_t resp, int& first_ctaid_x)
 {
     uint32_t ok, x = 0;
@@ -160,7 +162,8 @@ __device__ __forceinline__ bool clc_query(uint32_t resp, int& first_ctaid_x)
         "ld.shared.b128 r, [%2];\n\t"
         "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t"
-        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t"
+        "fence.proxy.async.shared::cta;\n\t}"
         : "=r"(ok), "+r"(x)
         : "r"(resp)
         : "memory");
