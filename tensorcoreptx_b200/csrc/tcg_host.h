@@ -1,5 +1,5 @@
 // tcg_host.h -- host-side services that the library's translation units share
-// (defined in tcgemm.cu; take_rows_error in tcg_rows.cu).
+// (defined in tcgemm.cu; the rows_error functions in tcg_rows.cu).
 #pragma once
 
 #include <cuda.h>
@@ -32,8 +32,9 @@ tcg_status encode_4d(CUtensorMap* map, CUtensorMapDataType dt, const void* base,
 bool dependent_launch();               // programmatic dependent launch (TCG_PDL)
 unsigned long long wait_timeout_ns();  // tcg_set_wait_timeout_ns
 
-// Read and clear the failure word of tcg_rows.cu's kernels on this device.
-tcg_status take_rows_error(unsigned long long* word);
+// The failure word of tcg_rows.cu's kernels on this device.
+cudaError_t read_rows_error(unsigned long long* word);
+cudaError_t clear_rows_error();
 
 }  // namespace host
 }  // namespace tcg

@@ -401,12 +401,15 @@ tcg_status gemm_s8(const int8_t* A, const int8_t* B, void* C, tcg_dtype c_type, 
 namespace tcg {
 namespace host {
 
-tcg_status take_rows_error(unsigned long long* word)
+cudaError_t read_rows_error(unsigned long long* word)
 {
-    cudaError_t e = cudaMemcpyFromSymbol(word, tcg::g_tcg_error_word, sizeof *word);
+    return cudaMemcpyFromSymbol(word, tcg::g_tcg_error_word, sizeof *word);
+}
+
+cudaError_t clear_rows_error()
+{
     const unsigned long long zero = 0;
-    if (e == cudaSuccess && *word != 0) e = cudaMemcpyToSymbol(tcg::g_tcg_error_word, &zero, sizeof zero);
-    return e == cudaSuccess ? TCG_SUCCESS : fail(e);
+    return cudaMemcpyToSymbol(tcg::g_tcg_error_word, &zero, sizeof zero);
 }
 
 }  // namespace host

@@ -1110,15 +1110,14 @@ tcg_status tcg_check_device_error(void* stream, uint64_t* word)
 {
     cudaError_t e = cudaStreamSynchronize(static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return cuda_fail(e);
-    unsigned long long w = 0;
-    e = cudaMemcpyFromSymbol(&w, tcg::g_tcg_error_word, sizeof w);
-    if (e != cudaSuccess) return cuda_fail(e);
+    // both words are read before either is cleared: a failure on the way loses none
+    unsigned long long w = 0, rows = 0;
     const unsigned long long zero = 0;
-    if (w != 0 && (e = cudaMemcpyToSymbol(tcg::g_tcg_error_word, &zero, sizeof zero)) != cudaSuccess)
-        return cuda_fail(e);
-    unsigned long long rows = 0;
-    const tcg_status s = tcg::host::take_rows_error(&rows);
-    if (s != TCG_SUCCESS) return s;
+    e = cudaMemcpyFromSymbol(&w, tcg::g_tcg_error_word, sizeof w);
+    if (e == cudaSuccess) e = tcg::host::read_rows_error(&rows);
+    if (e == cudaSuccess && w != 0) e = cudaMemcpyToSymbol(tcg::g_tcg_error_word, &zero, sizeof zero);
+    if (e == cudaSuccess && rows != 0) e = tcg::host::clear_rows_error();
+    if (e != cudaSuccess) return cuda_fail(e);
     if (w == 0) w = rows;
     if (word) *word = w;
     return w == 0 ? TCG_SUCCESS : TCG_ERR_TIMEOUT;

@@ -93,3 +93,24 @@ def test_wait_expiry_aborts_cleanly(name):
         assert L.tcg_check_device_error(stream, None) == 0
     finally:
         T().set_rows_tile(0, 0)
+
+
+def test_failures_of_both_kinds_of_kernel_are_reported_by_one_check():
+    """The dense kernels and these have a failure word each; a check reports the
+    dense one first and leaves neither behind."""
+    from tensorcoreptx_b200 import _native as nat
+    L = nat.lib()
+    call = layer(16384, 2304, 2048)
+    call()
+    stream = torch.cuda.current_stream().cuda_stream
+    assert L.tcg_check_device_error(stream, None) == 0
+    L.tcg_set_wait_timeout_ns(LIMIT_NS)
+    try:
+        call()
+    finally:
+        L.tcg_set_wait_timeout_ns(0)
+    assert L.tcg_selftest_wait_timeout(1_000_000, stream) == 0  # 1 ms, in the dense kernels' file
+    word = C.c_uint64(0)
+    assert L.tcg_check_device_error(stream, C.byref(word)) == nat.TCG_ERR_TIMEOUT
+    assert (word.value >> 32) == 1 and (word.value & 0xFF) in (0xFF, 0xFE)  # the self test's code
+    assert L.tcg_check_device_error(stream, C.byref(word)) == 0 and word.value == 0
