@@ -536,7 +536,9 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
     // kernel before this one wrote only the q operand and its scales, and let
     // this one start after its own wait: features and offsets may be read now.
     if (!p.early) grid_dependency_wait();
-    grid_launch_dependents();
+    // (by the warp that allocates: the next kernel's CTAs take what tensor memory
+    // is left only once every CTA here has its own, so neither waits for the other)
+    if (warp == 1) grid_launch_dependents();
     if (p.offsets && warp == 2) rows_table(p, C::kBQ, bound, cum);
     tc_fence_before();
     __syncthreads();
