@@ -133,7 +133,10 @@ tcg_status tcg_quantize_absmax_s4(const float* src, int8_t* dst_packed, int rows
  * major) to int8 codes of the same layout and scale[rows] (device floats):
  *   scale = max|x| / 127, code = round half away from zero (x * (1 / scale)),
  * every step in IEEE single precision; a row of zeros has scale 0 and codes 0,
- * a row with an infinity or NaN a scale that is not finite.  src and scale
+ * a row with an infinity or NaN a scale that is not finite.  Where 1 / scale
+ * would overflow (largest value below 3.7e-37) x and scale are taken 2^64 times
+ * as large; rows whose largest value is subnormal (below 1.2e-38) are not, and
+ * their codes are 0 and +-127.  src and scale
  * need their element's alignment only; rows of whole 16-byte vectors at a
  * 16-byte aligned src take the faster path.
  * tcg_dequantize_rows_s8 is the way back: dst = code * scale of the row in

@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) few_rows_kernel(const FewParam
 {
     extern __shared__ uint4 few_codes[];  // [kM][k / 16]
     __shared__ uint32_t part[kM][kFewWarps];
-    __shared__ float scale[kM], inv[kM];
+    __shared__ float scale[kM], inv[kM], tops[kM];
     constexpr int kN = RowVec<T>::kN;
     constexpr int kU = kFewLoads / kF;
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
@@ -86,15 +86,21 @@ __global__ void __launch_bounds__(kFewThreads, 2) few_rows_kernel(const FewParam
         for (int i = 0; i < kFewWarps; ++i) top = max(top, part[t][i]);
         const float absmax = __uint_as_float(top);
         scale[t] = __fdiv_rn(absmax, 127.f);
-        inv[t] = quant_inv(absmax, 127.f);
+        inv[t] = row_inv(absmax);
+        tops[t] = absmax;
     }
     __syncthreads();
     int8_t* codes = reinterpret_cast<int8_t*>(few_codes);
 #pragma unroll
     for (int m = 0; m < kM; ++m) {
-        const bool plain = scale[m] > 1e-32f && scale[m] < 2e36f;
-        for (int i = t; i < nv; i += kFewThreads)
-            row_codes<T>(x[static_cast<long long>(m) * nv + i], inv[m], plain, codes + static_cast<long long>(m) * p.k + i * kN);
+        const uint4* row = x + static_cast<long long>(m) * nv;
+        int8_t* to = codes + static_cast<long long>(m) * p.k;
+        if (row_plain(tops[m])) {
+            for (int i = t; i < nv; i += kFewThreads) plain_codes<T>(row[i], inv[m], to + i * kN);
+        } else {
+#pragma unroll 1
+            for (int i = t; i < nv; i += kFewThreads) any_codes<T>(row[i], inv[m], row_lift(tops[m]), to + i * kN);
+        }
     }
     __syncthreads();
 

@@ -117,8 +117,8 @@ __global__ void quantize_s4_kernel(const float* __restrict__ x, int8_t* __restri
 // ---- one scale per row ----------------------------------------------------
 //
 // codes[m][k] and scale[m] of each row m of fp32, fp16 or bf16 values, by the
-// arithmetic above with Q = 127 and the row's own absmax.  kGroup threads (a
-// warp or a block) take a row.  The row is read once: kVecs 16-byte vectors a
+// arithmetic above with Q = 127 and the row's own absmax, lifted as row_lift has it.  kGroup threads
+// (a warp or a block) take a row.  The row is read once: kVecs 16-byte vectors a
 // thread stay in registers between the absmax and the codes; what is longer is
 // read again, from L2.  A warp holds a row of up to 16 KB that way, with no
 // barrier and all of its loads in flight; a block per row is for few or longer
@@ -172,17 +172,21 @@ __global__ void __launch_bounds__(kRowThreads)
             for (int w = 1; w < kRowThreads / 32; ++w) m = max(m, wmax[w]);
         }
         const float absmax = __uint_as_float(m);
-        const float inv = quant_inv(absmax, 127.f);
-        const bool plain = absmax > 1e-30f && absmax < 3e38f;
+        const float inv = row_inv(absmax);
         if (!live) continue;
         if (t == 0) scale[row] = __fdiv_rn(absmax, 127.f);
-        if constexpr (kVecs > 0) {
+        const float lift = row_lift(absmax);
+        if (kVecs > 0 && row_plain(absmax)) {
 #pragma unroll
             for (int u = 0; u < kVecs; ++u)
-                if (t + u * kGroup < nv) row_codes<T>(v[u], inv, plain, orow + (t + u * kGroup) * kN);
-            for (int i = t + kVecs * kGroup; i < nv; i += kGroup) row_codes<T>(xv[i], inv, plain, orow + i * kN);
+                if (t + u * kGroup < nv) plain_codes<T>(v[u], inv, orow + (t + u * kGroup) * kN);
+            for (int i = t + kVecs * kGroup; i < nv; i += kGroup) plain_codes<T>(xv[i], inv, orow + i * kN);
+        } else if (kVecs > 0) {  // (rare: very small, very large or not finite values; read again)
+#pragma unroll 1
+            for (int i = t; i < nv; i += kGroup) any_codes<T>(xv[i], inv, lift, orow + i * kN);
         } else {
-            for (int i = t; i < k; i += kGroup) orow[i] = static_cast<int8_t>(quant_code(row_value(xr[i]), inv, 127.f));
+            for (int i = t; i < k; i += kGroup)
+                orow[i] = static_cast<int8_t>(quant_code(row_value(xr[i]) * lift, inv, 127.f));
         }
     }
 }

@@ -32,6 +32,30 @@ __device__ __forceinline__ uint32_t quant_word8(float4 v, float inv)
            ((static_cast<uint32_t>(quant_code(v.w, inv, 127.f)) & 0xFFu) << 24);
 }
 
+// How a row's values become codes: code = x * lift * inv, rounded.  The inverse of
+// a scale of 2^-128 or less (largest value below 127 * 2^-128 = 3.7e-37) passes
+// the range of fp32; rows up to 1e-30 and their scales are therefore taken 2^64
+// times as large, which is exact and changes no code where the plain inverse is
+// in range.  A row whose largest value is subnormal (below 2^-126) has no scale of
+// full precision either; it keeps the plain arithmetic, as the per-tensor quantiser
+// has it: its codes are +-127 and 0, a value's sign with the row's largest size.
+constexpr float kLift = 0x1p64f;
+
+// scale and inverse are ordinary numbers, or the row is all zeros (padding)
+__device__ __forceinline__ bool row_plain(float absmax)
+{
+    return absmax == 0.f || (absmax > 1e-30f && absmax < 3e38f);
+}
+__device__ __forceinline__ float row_lift(float absmax)
+{
+    return absmax >= 0x1p-126f && absmax <= 1e-30f ? kLift : 1.f;
+}
+__device__ __forceinline__ float row_inv(float absmax)
+{
+    const float s = __fmul_rn(__fdiv_rn(absmax, 127.f), row_lift(absmax));
+    return s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
+}
+
 template <class T>
 __device__ __forceinline__ float row_value(T v) { return static_cast<float>(v); }
 
@@ -82,38 +106,54 @@ __device__ __forceinline__ uint32_t sign_bytes(float a, float b)
     return r;
 }
 
-// Codes of 16 bytes.  `plain`: the row's scale and its inverse are ordinary
-// numbers, so |x| * inv is at most 127 (1 + 2^-22) and needs no clamp; then the
-// magnitude's code is read from the mantissa of (|x| * inv + 0.5) + 2^23, the
-// last sum rounded towards zero, and the signs are put in four bytes at a time.
-// The roundings are those of quant_code, without its conversions, compares and
-// selects: 7 instructions a value instead of 16, which bound the kernel (bf16
-// 8192 x 4096: 31 us).
 template <class T>
-__device__ __forceinline__ void row_codes(const uint4& v, float inv, bool plain, int8_t* out)
+__device__ __forceinline__ void store_codes(const uint32_t (&w)[RowVec<T>::kN / 4], int8_t* out)
+{
+    if constexpr (RowVec<T>::kN == 8)
+        *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
+    else
+        *reinterpret_cast<uint32_t*>(out) = w[0];
+}
+
+// Codes of 16 bytes of a plain row: |x| * inv is at most 127 (1 + 2^-22) and needs
+// no lift and no clamp; then the magnitude's code is read from the mantissa of
+// (|x| * inv + 0.5) + 2^23, the last sum rounded towards zero, and the signs are
+// put in four bytes at a time.  The roundings are those of quant_code, without its
+// conversions, compares and selects: 7 instructions a value instead of 16, which
+// bound the kernel (bf16 8192 x 4096: 31 us; 17 so, with any_codes in a loop of
+// its own -- 20 with both in every unrolled step).
+template <class T>
+__device__ __forceinline__ void plain_codes(const uint4& v, float inv, int8_t* out)
 {
     const RowVec<T> x(v);
     uint32_t w[RowVec<T>::kN / 4];
 #pragma unroll
     for (int i = 0; i < RowVec<T>::kN / 4; ++i) {
         const float* f = x.f + 4 * i;
-        if (plain) {
-            uint32_t u[4];
+        uint32_t u[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                u[j] = __float_as_uint(__fadd_rz(__fadd_rn(__fmul_rn(fabsf(f[j]), inv), 0.5f), 8388608.f));
-            const uint32_t m = __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
-            const uint32_t neg = __byte_perm(sign_bytes(f[0], f[1]), sign_bytes(f[2], f[3]), 0x5410);
-            const uint32_t minus = (0x80808080u - m) ^ 0x80808080u;  // -m in every byte (m <= 127: no borrow)
-            w[i] = (m & ~neg) | (minus & neg);
-        } else {
-            w[i] = quant_word8(make_float4(f[0], f[1], f[2], f[3]), inv);
-        }
+        for (int j = 0; j < 4; ++j)
+            u[j] = __float_as_uint(__fadd_rz(__fadd_rn(__fmul_rn(fabsf(f[j]), inv), 0.5f), 8388608.f));
+        const uint32_t m = __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
+        const uint32_t neg = __byte_perm(sign_bytes(f[0], f[1]), sign_bytes(f[2], f[3]), 0x5410);
+        const uint32_t minus = (0x80808080u - m) ^ 0x80808080u;  // -m in every byte (m <= 127: no borrow)
+        w[i] = (m & ~neg) | (minus & neg);
     }
-    if constexpr (RowVec<T>::kN == 8)
-        *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
-    else
-        *reinterpret_cast<uint32_t*>(out) = w[0];
+    store_codes<T>(w, out);
+}
+
+// Codes of 16 bytes of any row.
+template <class T>
+__device__ __forceinline__ void any_codes(const uint4& v, float inv, float lift, int8_t* out)
+{
+    const RowVec<T> x(v);
+    uint32_t w[RowVec<T>::kN / 4];
+#pragma unroll
+    for (int i = 0; i < RowVec<T>::kN / 4; ++i) {
+        const float* f = x.f + 4 * i;
+        w[i] = quant_word8(make_float4(f[0] * lift, f[1] * lift, f[2] * lift, f[3] * lift), inv);
+    }
+    store_codes<T>(w, out);
 }
 
 }  // namespace tcg

@@ -99,8 +99,11 @@ def quantize_rows_int8(x: torch.Tensor):
     """Absmax quantisation of each row (the last axis) of a float32, float16 or
     bfloat16 tensor: codes int8 of x's shape and scales float32 of its leading
     shape, scale = max|x| / 127 and codes rounded half away from zero, as
-    quantize_absmax_int8 does per tensor.  A row of zeros has scale 0; a row
-    with an infinity or a NaN gets a scale that is not finite."""
+    quantize_absmax_int8 does per tensor.  codes times scale are within half a
+    step, max|x| / 254, of x as long as max|x| is a normal fp32 number or 0 (in a
+    row of subnormal values, below 1.2e-38, they are 0 and +-max|x|).  A row of
+    zeros has scale 0; a row with an infinity or a NaN gets a scale that is not
+    finite."""
     return nat.torch_binding().quantize_rows(x)
 
 
