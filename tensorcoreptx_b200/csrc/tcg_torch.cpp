@@ -107,6 +107,8 @@ Tensor grouped_out(const OptTensor& out, const Tensor& A, std::initializer_list<
                 "out must be a contiguous CUDA tensor of shape [", A.size(0), ", ", N, "] and type ", type);
     same_device(A, "out", *out);
     for (const OptTensor& t : inputs) TORCH_CHECK(!t || !overlap(*out, *t), "out must not overlap the inputs");
+    TORCH_CHECK(!(at::GradMode::is_enabled() && out->requires_grad()), "out must not require grad");
+    out->unsafeGetTensorImpl()->bump_version();  // autograd: what was saved of it is stale
     return *out;
 }
 

@@ -18,8 +18,10 @@ at most 131056, so that the int32 sums are exact) or 8 (16 bits); the number of 
 ``offsets`` (int32, groups + 1 values on the device) are the ascending row
 bounds of the groups: group e is rows ``offsets[e]`` to ``offsets[e + 1] - 1``,
 any of them empty.  Rows outside every group (a padded batch) give zeros in a
-new result and are left alone in a given one (``out``, which overlaps no input).  Offsets that descend or exceed
-the rows are clamped, never followed out of range.
+new result and are left alone in a given one (``out``, which overlaps no input
+and, as with torch's own ``out=``, requires no gradient and counts as changed in
+place).  Offsets that descend or exceed the rows are clamped, never followed out
+of range.
 """
 from __future__ import annotations
 
@@ -90,6 +92,10 @@ def _grouped_out(out, A, inputs, M: int, N: int, dtype):
         raise RuntimeError(f"out must be a contiguous CUDA tensor of shape {(M, N)} and type {dtype}")
     _same_device(A, "out", out)
     _check(not any(_overlap(out, t) for t in inputs if t is not None), "out must not overlap the inputs")
+    _check(not (torch.is_grad_enabled() and out.requires_grad), "out must not require grad")
+    _check(torch.is_inference_mode_enabled() or not out.is_inference(),
+           "out must not be an inference tensor outside inference mode")
+    torch.autograd.graph.increment_version(out)  # autograd: what was saved of it is stale
     return out, 0
 
 
