@@ -201,7 +201,7 @@ def gemm_grouped(A: torch.Tensor, B: torch.Tensor, offsets: torch.Tensor, b_layo
                  out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """C[M,N] = rows of A[M,K] (float16 or bfloat16) times their group's matrix
     of B: [E,N,K] (b_layout="nk") or [E,K,N] ("kn"), fp32 sums, rounded once to
-    out_dtype (A's type, or float32)."""
+    out_dtype (float16, bfloat16 or float32; A's type unless given)."""
     _check(b_layout in ("nk", "kn"), "b_layout must be 'nk' or 'kn'")
     return nat.torch_binding().gemm_grouped(A, B, offsets, b_layout == "nk", out_dtype, out)
 
@@ -210,8 +210,8 @@ def gemm_grouped_wgrad(dC: torch.Tensor, A: torch.Tensor, offsets: torch.Tensor,
                        scale_a: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """dB[E,N,K], the gradient of gemm_grouped by B ("nk"): for each group the
     sum over its rows m of dC[m,N] (float16 or bfloat16) outer A[m,K], zero for
-    an empty group; fp32 sums, rounded once to out_dtype (dC's type, or
-    float32).  A has dC's type, or is the int8 codes of quantize_rows_int8 with
+    an empty group; fp32 sums, rounded once to out_dtype (float16, bfloat16 or
+    float32; dC's type unless given).  A has dC's type, or is the int8 codes of quantize_rows_int8 with
     their scales as scale_a[M], which stand for code * scale rounded to dC's
     type (a buffer of that size lives during the call).  (Swapping dC and A gives the "kn" gradient.)"""
     _check(dC.is_cuda and A.is_cuda, "dC and A must be CUDA tensors")
