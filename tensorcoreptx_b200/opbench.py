@@ -106,9 +106,10 @@ def main(argv=None):
         grouped = a.op == "linear_int8_grouped"
         B, sb = T.quantize_rows_int8(torch.randn(*((a.groups, N, K) if grouped else (N, K)), generator=g, device=dev))
         q, sq = T.quantize_rows_int8(X)
+        o = bounds()
         fn = {"gemm_int8_scaled": lambda: T.gemm_int8_scaled(q, B, sq, sb, out_dtype=torch.bfloat16),
               "linear_int8": lambda: T.linear_int8(X, B, sb),
-              "linear_int8_grouped": lambda: T.linear_int8_grouped(X, B, bounds(), sb)}[a.op]
+              "linear_int8_grouped": lambda: T.linear_int8_grouped(X, B, o, sb)}[a.op]
         work, unit = gemm_ops, "TOPS"
     elif a.op in ("gemm_grouped", "gemm_grouped_wgrad", "linear_train", "linear_train_int8"):
         X = torch.randn(M, K, generator=g, device=dev).bfloat16()
