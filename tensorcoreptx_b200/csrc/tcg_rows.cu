@@ -78,7 +78,7 @@ long long most_row_tiles(const RowsCall& c, int bq)
 //   kSub = 2:  10 + k-blocks x 0.54 (the tensor cores' rate) for the first whole
 //              wave, 4.5 + k-blocks x 0.54 for the others, at least 7 (128 KB of
 //              results at the rate at which all SMs write, 14 bytes a cycle each)
-// Example: int8 512 x 4096 x 4096 64 rows 13.4 (model 15.1), 128 rows 12.9
+// Example: int8 512 x 4096 x 4096 64 rows 13.4 (model 16.3), 128 rows 12.9
 // (13.6), 256 rows 29.1 (27.3); 100 x 4096 x 4096: 32 rows 10.8, 64 rows on two
 // CTAs 9.0, 128 rows on four 8.5.
 RowsPlan choose_plan(const RowsCall& c, bool weight, int kblock, int sms)

@@ -38,11 +38,12 @@
 // Warps: 0 TMA producer, 1 MMA issuer, 2..9 epilogue (two per tensor-memory lane
 // quarter).  Every wait on an mbarrier is bounded (tcg_wait.cuh).
 //
-// What bounds it (B200): one row of 4096 x 4096 int8 6.2 us, of which loading,
-// multiplying and adding up are 3 and the rest launch and synchronisation;
-// experts' weights of 64 x 2048 x 4096 int8 at 6.0 TB/s of 6.5; int8 16384 x 8192
-// x 8192 2.8-2.9 POPS and bf16 8192 x 8192 x 4096 1.48-1.57 PFLOP/s under the
-// power limit, as cuBLAS.
+// What bounds it (B200): few rows, start and exchange, then the weights' bytes
+// (eight rows of 4096 x 4096 int8, quantising included, 8.5 us where the bytes are
+// 2.6; experts' weights of 64 x 2048 x 4096 int8 at 6.0 TB/s of 6.5); many rows,
+// the tensor cores, under the power limit after some ms: int8 16384 x 8192 x 8192
+// 714 us (3.08 POPS), 820 sustained; bf16 8192 x 8192 x 4096 366 us (1.50 PFLOP/s),
+// 422 sustained (the library's product 350 and 406).
 #pragma once
 
 #include <cuda_bf16.h>

@@ -9,6 +9,9 @@ grouped by expert, and layers that train through them.
 * ``linear``, ``linear_grouped``: differentiable 16-bit layers, which with
   ``save="int8"`` keep an 8-bit copy of their input for the backward pass.
 
+Only the layers differentiate; the results of the others, like those of the
+package's dense products, carry no gradient to inputs that require one.
+
 Like the other entries they check their arguments (``RuntimeError``), return
 new tensors on the inputs' device, run asynchronously on that device's current
 stream, and can be captured into CUDA graphs.  There is no CPU or library
@@ -242,7 +245,8 @@ def linear(x: torch.Tensor, W: torch.Tensor, save: str = "input") -> torch.Tenso
     differentiable by x and W.  save="int8" keeps x for the backward pass as
     int8 codes with a scale per row, half of its bytes (the backward pass widens
     one layer's codes at a time): the output and x's gradient are unchanged, W's
-    gradient is that of the codes."""
+    gradient is that of code * scale rounded to x's type (half a step of that
+    type on top of the codes' half step)."""
     _check(save in ("input", "int8"), "save must be 'input' or 'int8'")
     return nat.torch_binding().linear(x, W, None, save == "int8")
 
